@@ -42,6 +42,7 @@ from .attention import (
     HAS_FLASH_ATTN,
     HAS_TRITON,
 )
+from .speculative import draft_layout, paged_draft_attention, verify_drafts, commit_drafts, MAX_DRAFT_NODES
 from .model_runner import ModelRunner, ModelRunnerConfig, DecodeState
 from .qwen3_paged import Qwen3PagedConfig, Qwen3PagedModel
 from . import _native
@@ -53,5 +54,6 @@ __all__ = [
     "paged_decode", "paged_decode_shared_prefix", "find_prefix_groups", "find_prefix_groups_anywhere", "PrefixGroups", "shared_prefix_descriptors", "prepare_prefix_groups", "paged_prefill", "choose_partition", "choose_launch", "reserve_decode_workspace", "sizing_graph_workspace",
     "decode_workspace_bytes", "release_decode_workspaces", "check_block_tables",
     "HAS_FLASH_ATTN", "HAS_TRITON",
+    "draft_layout", "paged_draft_attention", "verify_drafts", "commit_drafts", "MAX_DRAFT_NODES",
     "ModelRunner", "ModelRunnerConfig", "Qwen3PagedConfig", "Qwen3PagedModel",
 ]

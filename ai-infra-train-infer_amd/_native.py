@@ -25,6 +25,7 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _ptr = ctypes.c_void_p
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> (restype, argtypes); mirrors include/paged_attn.h one to one
 SIGNATURES = {
@@ -63,6 +64,15 @@ SIGNATURES = {
     "pa_decode_advance": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr]),
     "pa_prefill_metadata": (_int, [_ptr, _ptr, _ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr]),
     "pa_slot_mapping": (_int, [_ptr, _ptr, _ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _ptr]),
+    "pa_draft_layout": (_int, [_ptr, _i64, _ptr, _ptr, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _ptr]),
+    "pa_verify_workspace_bytes": (_i64, [_i64, _i64, _i64]),
+    "pa_verify_drafts": (_int, [_ptr, _int, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _int, _i64, _i64, _f64, _f64,
+                                _i64, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]),
+    "pa_draft_commit": (_int, [_ptr, _i64, _i64, _i64, _ptr, _ptr, _i64, _ptr, _i64, _i64, _ptr, _ptr, _i64, _ptr, _ptr, _i64,
+                               _i64, _i64, _i64, _ptr]),
+    "pa_draft_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "pa_draft_attention": (_int, [_ptr, _int, _i64, _ptr, _ptr, _ptr, _ptr, _int, _ptr, _i64, _i64, _ptr, _ptr, _ptr, _i64, _ptr,
+                                  _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i64, _i64, _ptr, _i64, _int, _ptr]),
     "pa_check_tables": (_int, [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _ptr]),
 }
 

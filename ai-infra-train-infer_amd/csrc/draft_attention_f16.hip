@@ -1,0 +1,11 @@
+// Instantiations of the drafted-token attention kernel (one translation unit per cache and product type, so
+// that they compile side by side).
+#include "draft_attention_kernel.hpp"
+
+namespace pa {
+
+int launch_draft_f16(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st) {
+  return launch_draft<KV_F16, CT_F16>(p, head_dim, col_tiles, grid, st);
+}
+
+}  // namespace pa

@@ -471,6 +471,115 @@ int pa_check_tables(const int32_t* block_tables, int64_t bt_stride, int64_t tabl
                     const int32_t* context_lens, int64_t batch, int64_t block_size,
                     int64_t num_blocks, int32_t* counts, void* stream);
 
+/* ---- speculative decoding -------------------------------------------------------------------------
+ * A step checks several drafted tokens of every sequence in one forward pass of the target model.  A row
+ * drafts a tree of at most PA_MAX_DRAFT_NODES nodes: node 0 is the last accepted token (whose K and V are not
+ * cached yet), parents[i] < i the node that node i follows; a chain is parents[i] = i - 1.  A step is
+ *   pa_draft_layout           positions, cache slots and ancestors of the nodes
+ *   (the model's layers)      pa_qk_norm_rope_store or pa_kv_store writes node i at cache position context_len + i,
+ *   pa_draft_attention        every node attends to the committed tokens and its own ancestors
+ *   pa_verify_drafts          the nodes that the target accepts, and the token after them
+ *   pa_draft_commit           their K and V rows move to consecutive positions
+ * with context_lens counting the committed tokens throughout, num_nodes (optional, int32 [batch]) how many
+ * nodes a row drafts (0: an inactive row, as in a padded batch; NULL: all of them).
+ * Replaces: the draft / target decoder's verification loop (src/inference/speculative.py), which runs a
+ * HuggingFace model over chains and keeps no paged cache.
+ */
+#define PA_MAX_DRAFT_NODES 256
+
+/*
+ * Positions, cache slots and ancestor sets of the drafted nodes.
+ *   parents              int32, rows parents_stride apart; parents_stride 0: one tree of `nodes` for every row.
+ *                        A parent outside [0, i) makes node i a root that descends from itself alone.
+ *   positions            int64 [batch, nodes] = context_len + depth (0 for nodes past num_nodes)
+ *   slots                int32 [batch, nodes], the slot of cache position context_len + i; -1 for nodes past
+ *                        num_nodes, outside the table or the pool (the KV writers skip those).  NULL allowed
+ *                        with block_tables NULL.
+ *   tree_mask            uint64 [batch or, with one tree, 1][nodes][ceil(nodes / 64)]: bit j % 64 of word j / 64
+ *                        is set where node j is node i or one of its ancestors
+ */
+int pa_draft_layout(const int32_t* parents, int64_t parents_stride, const int32_t* context_lens,
+                    const int32_t* num_nodes, const int32_t* block_tables, int64_t bt_stride,
+                    int64_t table_width, int64_t* positions, int32_t* slots, uint64_t* tree_mask,
+                    int64_t batch, int64_t nodes, int64_t block_size, int64_t num_blocks, void* stream);
+
+/*
+ * Which drafted nodes the target accepts, and the token after the last of them.  Per row, from node 0 on, the
+ * children of an accepted node are tried in index order against the target's distribution after that node:
+ * p = softmax(logits / temperature), with top_p < 1 restricted to the tokens that pa_sample keeps.
+ *   no draft_probs       child c passes iff uniforms[c] * (1 - mass of the siblings refused before) < p(token_c);
+ *                        a token offered twice under one node counts once
+ *   draft_probs          chains only: uniforms[c] * q(token_c) < p(token_c), q the row of c's parent: the
+ *                        distribution the token was drawn from
+ *   temperature <= 0     token_c is the first maximum of its parent's logits
+ * The first child that passes is accepted and its own children come next.  When none passes, the token that
+ * follows is drawn by inversion of uniforms[0] in index order from what is left: p without the refused children,
+ * max(p - q, 0), or p after a leaf (and where nothing is left); greedy: the first maximum.  So the emitted tokens
+ * are distributed as pa_sample's.  Sums, thresholds and comparisons are in 64 bits.
+ *   logits               [batch, nodes, vocab] f16 / bf16 / f32, strides in elements; NaN counts as -inf
+ *   tokens               int64 [batch, nodes]; node 0's is not read; ids outside the vocabulary are never accepted
+ *   uniforms             float [batch, nodes] in [0, 1); NULL allowed for greedy
+ *   parents              int32 as for pa_draft_layout; NULL: a chain
+ *   draft_probs          [batch, nodes - 1, vocab] of draft_dtype, strides in elements, NULL: the drafts are points
+ *   out_tokens           int64 [batch, nodes]: the accepted tokens, then the one that follows, then -1
+ *   out_counts           int32 [batch]: tokens emitted = nodes kept (node 0 and the accepted ones); 0: inactive row
+ *   out_path             int32 [batch, nodes]: the nodes kept, in ascending order, then -1
+ *   workspace            >= pa_verify_workspace_bytes(...) bytes, 256-byte aligned
+ * vocab at most 2^24.
+ */
+int64_t pa_verify_workspace_bytes(int64_t batch, int64_t nodes, int64_t vocab);
+int pa_verify_drafts(const void* logits, int dtype, int64_t row_stride, int64_t batch_stride,
+                     const int64_t* tokens, const float* uniforms, const int32_t* parents,
+                     int64_t parents_stride, const int32_t* num_nodes, const void* draft_probs,
+                     int draft_dtype, int64_t draft_row_stride, int64_t draft_batch_stride,
+                     double temperature, double top_p, int64_t batch, int64_t nodes, int64_t vocab,
+                     int64_t* out_tokens, int32_t* out_counts, int32_t* out_path, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
+/*
+ * The kept nodes' K and V rows move, in every layer, from cache position context_len + path[j] to
+ * context_len + j, j in [1, counts[row]); new_lens = context_lens + counts.
+ *   pool                 [2 x layers][num_blocks][block_size][row_bytes], all K planes before all V planes,
+ *                        planes plane_stride_bytes apart
+ *   k_scale, v_scale     fp8 pools: [layers][num_blocks][block_size] float, layers scale_stride apart; else NULL
+ *   path, counts         as pa_verify_drafts writes them: ascending nodes, so that path[j] >= j
+ *   new_lens             int32 [batch], not context_lens itself
+ * Positions outside a row's table or the pool are skipped.  The rows' drafted positions must not share blocks.
+ */
+int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int64_t row_bytes, float* k_scale,
+                    float* v_scale, int64_t scale_stride, const int32_t* block_tables, int64_t bt_stride,
+                    int64_t table_width, const int32_t* context_lens, const int32_t* path,
+                    int64_t path_stride, const int32_t* counts, int32_t* new_lens, int64_t batch,
+                    int64_t nodes, int64_t block_size, int64_t num_blocks, void* stream);
+
+/*
+ * Attention of the drafted nodes over the paged cache: node i of row b attends to the context_lens[b] committed
+ * tokens and to the nodes j < num_nodes[b] of its mask, whose K and V lie at cache positions context_lens[b] + j:
+ *   out[b, i, h, :] = softmax_j(scale * q[b, i, h, :] . K[b, j, h / G, :]) @ V[b, :, h / G, :]
+ * A node that sees nothing (no context and an empty mask), nodes past num_nodes and rows of negative context
+ * get zeros.  What a node does not see never reaches its output, NaN and infinities included.
+ *   q, out               [batch, nodes, num_q_heads, head_dim] f16 / bf16 / f32, node stride in elements (rows of
+ *                        the batch nodes x stride apart), 16-byte aligned rows
+ *   tree_mask            as pa_draft_layout writes it, rows mask_stride words apart, 0: one tree for every row
+ *   max_partitions       1: one pass; > 1: the tokens of a row (committed and drafted) are cut every
+ *                        partition_size tokens as in pa_decode, and a second launch merges
+ *   workspace            >= pa_draft_workspace_bytes(...) bytes, 256-byte aligned, when max_partitions > 1
+ *   col_tiles            16-row tiles of (node, query head) rows of one KV head that a wave multiplies with a
+ *                        K/V tile: 1, 2, or 0 = the launch's own choice; the result does not depend on it
+ * Cache, tables, scales and sizes as for pa_decode.  16-bit caches and queries of one type are multiplied as they
+ * are, everything else as fp16; accumulation and softmax statistics are fp32.
+ */
+int64_t pa_draft_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_q_heads, int64_t head_dim,
+                                 int64_t max_partitions);
+int pa_draft_attention(const void* q, int q_dtype, int64_t q_stride, const void* k_cache, const void* v_cache,
+                       const float* k_scale, const float* v_scale, int kv_dtype, const int32_t* block_tables,
+                       int64_t bt_stride, int64_t table_width, const int32_t* context_lens,
+                       const int32_t* num_nodes, const uint64_t* tree_mask, int64_t mask_stride, void* out,
+                       int64_t out_stride, int64_t batch, int64_t nodes, int64_t num_q_heads,
+                       int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks,
+                       float scale, int64_t partition_size, int64_t max_partitions, void* workspace,
+                       int64_t workspace_bytes, int col_tiles, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,547 @@
+"""Speculative decoding on the GPU: layout, attention, verification and commit of drafted trees against the 64-bit
+oracle, one operator at a time and as a step, eager, captured and on several streams."""
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import speculative_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+FP8 = torch.float8_e4m3fn
+DT = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32, "fp8": FP8}
+
+
+def make_parents(kind, nodes, rng):
+    if kind == "chain":
+        return [i - 1 for i in range(nodes)]
+    if kind == "star":
+        return [-1] + [0] * (nodes - 1)
+    return [-1] + [rng.randrange(max(0, i - 6), i) if kind == "deep" else rng.randrange(i) for i in range(1, nodes)]
+
+
+# ---------------------------------------------------------------------------------------------- layout
+
+@pytest.mark.parametrize("nodes", [1, 2, 5, 63, 64, 65, 128, 129, 256])
+@pytest.mark.parametrize("shared", [False, True])
+def test_layout_equals_the_oracle(pa, gpu, nodes, shared):
+    rng = random.Random(nodes)
+    bs, blocks = 8 if nodes % 2 else 16, 400
+    batch = 6
+    kinds = ["chain", "star", "deep", "tree", "tree", "deep"]
+    parents = [make_parents(kinds[0 if shared else b], nodes, rng) for b in range(batch)]
+    if not shared:
+        parents[3] = [rng.choice([-1, i, i + 3, 300, -7]) if rng.random() < 0.2 else p for i, p in enumerate(parents[3])]   # malformed
+    lens = [0, 7, 100, 33, 4000, -1]
+    real = [nodes, 0, max(1, nodes // 2), nodes, nodes + 9, nodes]
+    width = 40
+    tables = [[rng.randrange(blocks) for _ in range(width)] for _ in range(batch)]
+    tables[2][100 // bs] = -1
+    tables[3][33 // bs] = blocks
+    wide = torch.full((batch, width + 5), 3, dtype=torch.int32)
+    wide[:, :width] = torch.tensor(tables, dtype=torch.int32)
+    par = torch.tensor(parents[0] if shared else parents, dtype=torch.int32)
+    for use_real in (False, True):
+        pos, slots, mask = pa.draft_layout(par.to(gpu), torch.tensor(lens, dtype=torch.int32, device=gpu), wide.to(gpu)[:, :width],
+                                           bs, blocks, torch.tensor(real, dtype=torch.int32, device=gpu) if use_real else None)
+        assert mask.shape == (1 if shared else batch, nodes, (nodes + 63) // 64)
+        for b in range(batch):
+            n = 0 if lens[b] < 0 else min(real[b], nodes) if use_real else nodes
+            want_pos, want_slots, sets = so.layout(parents[b], lens[b], n, tables[b], bs, blocks)
+            assert pos[b].tolist() == want_pos and slots[b].tolist() == want_slots, b
+            assert torch.equal(mask[0 if shared else b].cpu(), so.mask_words(sets, nodes)), b
+    pos2, none, _ = pa.draft_layout(par.to(gpu), torch.tensor(lens, dtype=torch.int64, device=gpu))
+    assert none is None and pos2.shape == (batch, nodes)
+
+
+def test_layout_refusals(pa, gpu):
+    par, lens = torch.tensor([-1, 0], dtype=torch.int32, device=gpu), torch.tensor([4, 5], dtype=torch.int32, device=gpu)
+    with pytest.raises(RuntimeError, match="1 to 256"):
+        pa.draft_layout(torch.zeros(257, dtype=torch.int32, device=gpu), lens)
+    with pytest.raises(RuntimeError, match="parents"):
+        pa.draft_layout(torch.zeros(3, 2, dtype=torch.int32, device=gpu), lens)
+    with pytest.raises(RuntimeError, match="num_blocks"):
+        pa.draft_layout(par, lens, torch.zeros(2, 4, dtype=torch.int32, device=gpu))
+    with pytest.raises(RuntimeError, match="num_nodes"):
+        pa.draft_layout(par, lens, num_nodes=torch.zeros(3, dtype=torch.int32, device=gpu))
+    with pytest.raises(RuntimeError, match="cpu"):
+        pa.draft_layout(par.cpu(), lens)
+    empty = pa.draft_layout(par, lens[:0])
+    assert empty[0].shape == (0, 2) and empty[1] is None
+
+
+# ---------------------------------------------------------------------------------------------- attention
+
+class Pool:
+    """A poisoned paged cache in which the rows' committed and drafted tokens are written, CPU side."""
+
+    def __init__(self, seed, lens, real, hkv, dim, block, cache, spread=1.0):
+        g = torch.Generator().manual_seed(seed)
+        need = [(c + n + block - 1) // block for c, n in zip(lens, real)]
+        self.blocks, self.block = sum(need) + 4, block
+        order = torch.randperm(self.blocks, generator=g).tolist()
+        self.tables = torch.full((len(lens), max(need + [1]) + 2), -1, dtype=torch.int32)
+        shape = (self.blocks, block, hkv, dim)
+        self.kf = torch.randn(shape, generator=g) * spread
+        self.vf = torch.randn(shape, generator=g)
+        self.ks = self.vs = None
+        if cache == "fp8":
+            self.ks, self.vs = 448.0 / self.kf.abs().amax((2, 3)), 448.0 / self.vf.abs().amax((2, 3))
+            self.k, self.v = (self.kf * self.ks[..., None, None]).to(FP8), (self.vf * self.vs[..., None, None]).to(FP8)
+        else:
+            self.k, self.v = self.kf.to(DT[cache]), self.vf.to(DT[cache])
+        used = torch.zeros(self.blocks, block, dtype=torch.bool)
+        at = 0
+        for b, k in enumerate(need):
+            ids = order[at:at + k]
+            at += k
+            self.tables[b, :k] = torch.tensor(ids, dtype=torch.int32)
+            pos = torch.arange(lens[b] + real[b])
+            used[torch.tensor(ids + [0])[pos // block], pos % block] = True
+        for t in (self.k, self.v):
+            if t.dtype == FP8:
+                t.view(torch.uint8)[~used] = 0x7F
+            else:
+                t[~used] = float("nan")
+        if self.ks is not None:
+            self.ks[~used] = float("nan")
+            self.vs[~used] = float("nan")
+
+    def device(self, gpu):
+        to = lambda t: None if t is None else t.to(gpu)
+        return to(self.k), to(self.v), to(self.tables), to(self.ks), to(self.vs)
+
+
+def bound(out, spread, weight, p_type, out_type):
+    """How far one output may be off, element by element.  A probability is rounded to p_type (half a step) and its
+    exponent carries the fp32 error of the score: a dot product of up to 128 terms of |q k| * scale <= 12, 130 * 2^-24 * 12
+    = 2^-13.4, taken as 2^-13.  Probabilities below fp16's smallest normal number are off by up to 2^-25 of the reference
+    point's, and the row sum is at least 2^-0 of it.  Then one rounding of the output."""
+    eps = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+    tiny = 2.0 ** -25 if p_type == torch.float16 else 0.0
+    return (eps[p_type] + 2.0 ** -13) * spread + tiny * weight + eps[out_type] * (out.abs() + spread * 2.0 ** -7) + 2.0 ** -25
+
+
+def check_attention(pa, gpu, seed, lens, nodes, hq, hkv, dim, block, cache, q_type, kind="tree", real=None, partitions=(None,),
+                    shared=False, q_view=None, change=None, sets_of=None, scale=None, spread=1.0, tweak_q=None):
+    rng = random.Random(seed)
+    batch = len(lens)
+    real_ = [nodes] * batch if real is None else real
+    pool = Pool(seed, lens, real_, hkv, dim, block, cache, spread)
+    if change:
+        change(pool)
+    parents = [make_parents(kind, nodes, rng)] * batch if shared else [make_parents(kind, nodes, rng) for _ in range(batch)]
+    sets = [so.ancestors(p) for p in parents]
+    if sets_of:
+        sets = sets_of(sets)
+    mask = torch.stack([so.mask_words(s, nodes) for s in (sets[:1] if shared else sets)])
+    g = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(batch, nodes, hq, dim, generator=g).to(DT[q_type])
+    if tweak_q:
+        tweak_q(q)
+    scale = dim ** -0.5 if scale is None else scale
+    p_type = torch.bfloat16 if cache == "bf16" and q_type == "bf16" else torch.float16
+    # what the kernel multiplies: queries of another type than the cache go through fp16
+    q_eff = q if p_type == torch.bfloat16 or q_type == "fp16" else q.to(torch.float16)
+    k, v, tables, ks, vs = pool.device(gpu)
+    qd = q.to(gpu) if q_view is None else q_view(q.to(gpu))
+    real_t = None if real is None else torch.tensor(real, dtype=torch.int32, device=gpu)
+    outs = []
+    for part in partitions:
+        out = pa.paged_draft_attention(qd, k, v, tables, torch.tensor(lens, dtype=torch.int32, device=gpu), mask.to(gpu), scale,
+                                       k_scale=ks, v_scale=vs, num_nodes=real_t, partition_size=part)
+        assert out.shape == qd.shape and out.dtype == q.dtype
+        outs.append(out.float().cpu().view(batch, nodes, hq, dim))
+    for b in range(batch):
+        n = real_[b]
+        kr = so.row_kv(pool.k, pool.ks, pool.tables[b].tolist(), lens[b] + n, block)
+        vr = so.row_kv(pool.v, pool.vs, pool.tables[b].tolist(), lens[b] + n, block)
+        want, spread_, weight = so.attention(q_eff[b], kr, vr, lens[b], sets[b], n, scale)
+        for part, out in zip(partitions, outs):
+            far = (out[b].double() - want).abs()
+            may = bound(want, spread_, weight, p_type, DT[q_type])
+            assert not torch.isnan(out[b]).any(), (b, part)
+            assert (far <= may).all(), (b, part, float((far / may).max()))
+    return outs
+
+
+HEADS = [(2, 2), (4, 2), (6, 2), (16, 2), (5, 1), (16, 8)]
+
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16"), ("fp8", "bf16"), ("bf16", "fp16"),
+                                          ("fp16", "bf16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_types(pa, gpu, cache, q_type, dim):
+    check_attention(pa, gpu, 11, [0, 1, 40, 200, 333], 7, 4, 2, dim, 16, cache, q_type, partitions=(None, 0, 32, 128))
+
+
+@pytest.mark.parametrize("hq,hkv", HEADS)
+@pytest.mark.parametrize("nodes", [1, 3, 8, 17])
+def test_attention_head_layouts_and_tree_sizes(pa, gpu, hq, hkv, nodes):
+    check_attention(pa, gpu, 100 * nodes + hq, [5, 64, 150], nodes, hq, hkv, 64, 8, "fp16", "fp16", partitions=(None, 0, 64))
+
+
+@pytest.mark.parametrize("nodes", [33, 64, 65, 130, 256])
+@pytest.mark.parametrize("kind", ["chain", "star", "deep"])
+def test_attention_large_trees(pa, gpu, nodes, kind):
+    cache, q_type = ("bf16", "bf16") if nodes % 2 else ("fp8", "fp16")
+    check_attention(pa, gpu, nodes, [0, 77], nodes, 2, 1, 64, 16, cache, q_type, kind=kind, partitions=(0, 64), shared=nodes == 64)
+
+
+@pytest.mark.parametrize("base", [0, 1, 15, 16, 31, 32, 33, 95, 96, 97, 127, 128, 129, 160])
+def test_attention_every_offset_of_the_tree_in_a_tile(pa, gpu, base):
+    check_attention(pa, gpu, base, [base, base + 64], 6, 2, 1, 64, 8, "fp16", "fp16", partitions=(0, 32, 96))
+    check_attention(pa, gpu, base, [base], 40, 2, 2, 128, 16, "fp8", "fp16", partitions=(0, 32))
+
+
+@pytest.mark.parametrize("block", [8, 16, 64, 256])
+def test_attention_block_sizes(pa, gpu, block):
+    check_attention(pa, gpu, block, [3, 250, 511], 5, 4, 2, 128, block, "fp8" if block > 16 else "bf16", "bf16", partitions=(None, 128))
+
+
+def test_attention_padded_rows_and_short_trees(pa, gpu):
+    lens, real = [40, 0, 17, 90, 8], [6, 0, 0, 1, 3]
+    outs = check_attention(pa, gpu, 5, lens, 6, 4, 2, 128, 16, "fp16", "fp16", real=real, partitions=(None, 0, 32))
+    for out in outs:
+        for b, n in enumerate(real):
+            assert (out[b, n:] == 0).all()
+    # a negative length is no row
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device=gpu)
+    q = torch.ones(2, 3, 2, 64, dtype=torch.float16, device=gpu)
+    t = torch.zeros(2, 2, dtype=torch.int32, device=gpu)
+    m = torch.ones(1, 3, 1, dtype=torch.int64, device=gpu)
+    out = pa.paged_draft_attention(q, k, k + 1, t, torch.tensor([-5, 4], dtype=torch.int32, device=gpu), m, 1.0)
+    assert (out[0] == 0).all() and (out[1] == 1).all()
+
+
+def test_attention_masks_that_leave_a_node_nothing(pa, gpu):
+    def some_empty(sets):
+        return [[set() if (i + b) % 2 else s for i, s in enumerate(row)] for b, row in enumerate(sets)]
+    outs = check_attention(pa, gpu, 21, [0, 0, 70], 10, 4, 2, 64, 16, "bf16", "bf16", partitions=(0, 32), sets_of=some_empty)
+    for out in outs:
+        assert (out[0, 1::2] == 0).all() and (out[1, ::2] == 0).all()
+        assert (out[2] != 0).any(-1).all()            # the committed tokens remain
+
+
+def test_attention_any_mask_is_taken_as_it_is(pa, gpu):
+    """Not a tree: a node sees later nodes, itself not, all of them."""
+    def odd(sets):
+        return [[{len(row) - 1 - i} | ({0, 2} if i % 3 else set(range(len(row)))) for i in range(len(row))] for row in sets]
+    check_attention(pa, gpu, 22, [0, 33], 12, 2, 2, 128, 16, "fp16", "fp16", partitions=(0, 32), sets_of=odd)
+
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16")])
+@pytest.mark.parametrize("nodes", [6, 24])
+def test_attention_nan_and_infinity_stay_on_their_branch(pa, gpu, cache, q_type, nodes):
+    """K and V of one drafted node hold NaN and infinities: only the nodes that see it may show it."""
+    lens, wild = [0, 45], 2
+    rng = random.Random(9)
+    sets = so.ancestors(make_parents("star", nodes, rng))
+    clean = Pool(31, lens, [nodes] * 2, 2, 128, 16, cache)
+    dirty = Pool(31, lens, [nodes] * 2, 2, 128, 16, cache)
+    for b, base in enumerate(lens):
+        pos = base + wild
+        at = (int(dirty.tables[b, pos // 16]), pos % 16)
+        if cache == "fp8":
+            dirty.k.view(torch.uint8)[at] = 0x7F
+            dirty.v.view(torch.uint8)[at] = 0xFF
+        else:
+            dirty.k[at], dirty.v[at] = float("inf"), float("nan")
+            dirty.v[at][0, :7] = -float("inf")
+    mask = so.mask_words(sets, nodes)[None].to(gpu)
+    q = torch.randn(2, nodes, 4, 128, generator=torch.Generator().manual_seed(8)).to(DT[q_type]).to(gpu)
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    for part in (0, 32):
+        outs = []
+        for pool in (clean, dirty):
+            k, v, t, ks, vs = pool.device(gpu)
+            outs.append(pa.paged_draft_attention(q, k, v, t, lens_t, mask, 128 ** -0.5, ks, vs, partition_size=part).float())
+        others = [i for i in range(nodes) if i != wild]
+        assert not torch.isfinite(outs[1][:, wild]).all()
+        assert torch.isfinite(outs[1][:, others]).all()
+        # the same values, summed key by key instead of by the matrix pipe: within the roundings of one output
+        step = 2.0 ** -7 if q_type == "bf16" else 2.0 ** -10
+        torch.testing.assert_close(outs[1][:, others], outs[0][:, others], rtol=step, atol=2.0 ** -12)
+
+
+def test_attention_scores_far_from_zero(pa, gpu):
+    """Row maxima of hundreds, below zero for some rows from the first tile on, above it for others."""
+    def lean(q):
+        q[:, ::2] = q[:, ::2].abs() * 3
+        q[:, 1::2] = -q[:, 1::2].abs() * 3
+    def positive(pool):
+        live = ~torch.isnan(pool.k)
+        pool.k = torch.where(live, pool.k.abs() + 0.5, pool.k)
+    # scores up to 128 * 9 * 2 * scale: 130 * 2^-24 of 205 is 2^-9.3 in the exponent, which bound() does not cover; halved
+    # here by the scale so that its 2^-13 holds: |q k| scale = 12
+    check_attention(pa, gpu, 77, [0, 64, 200], 6, 2, 1, 128, 16, "fp16", "fp16", partitions=(0, 32), change=positive, tweak_q=lean,
+                    scale=12 / 400)
+    check_attention(pa, gpu, 78, [130], 5, 2, 1, 64, 16, "bf16", "bf16", partitions=(0, 64), spread=2.0, scale=0.11)
+
+
+def test_attention_takes_views_and_flat_queries(pa, gpu):
+    view = lambda q: torch.cat([q, q * 0 + 7], 2)[:, :, :q.shape[2]]
+    check_attention(pa, gpu, 41, [9, 60], 5, 4, 2, 64, 16, "fp16", "fp16", q_view=view)
+    check_attention(pa, gpu, 42, [9, 60], 5, 4, 2, 64, 16, "fp16", "fp16", q_view=lambda q: q.reshape(10, 4, 64))
+    check_attention(pa, gpu, 43, [9, 60], 5, 4, 2, 64, 16, "fp16", "fp16", q_view=lambda q: q.transpose(2, 3).contiguous().transpose(2, 3))
+    # a flat view of a packed projection, shifted off 16 bytes
+    check_attention(pa, gpu, 44, [9, 60], 5, 4, 2, 64, 16, "fp16", "fp16",
+                    q_view=lambda q: torch.cat([q.reshape(10, 256)[:, :1], q.reshape(10, 256)], 1)[:, 1:].view(10, 4, 64))
+
+
+def test_attention_corrupt_tables_stay_inside_the_pool(pa, gpu):
+    k = torch.randn(6, 16, 2, 64, device=gpu).half()
+    t = torch.tensor([[9, -3, 1 << 30], [2, 3, 4]], dtype=torch.int32, device=gpu)
+    q = torch.randn(2, 3, 4, 64, device=gpu).half()
+    m = torch.full((1, 3, 1), 7, dtype=torch.int64, device=gpu)
+    for part in (0, 32):
+        # the second row's tokens need more columns than the table has
+        out = pa.paged_draft_attention(q, k, k, t, torch.tensor([40, 100], dtype=torch.int32, device=gpu), m, 0.1, partition_size=part)
+        assert torch.isfinite(out.float()).all()
+
+
+def test_attention_refusals(pa, gpu):
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device=gpu)
+    q = torch.zeros(2, 3, 4, 64, dtype=torch.float16, device=gpu)
+    t = torch.zeros(2, 2, dtype=torch.int32, device=gpu)
+    lens = torch.tensor([4, 5], dtype=torch.int32, device=gpu)
+    m = torch.ones(2, 3, 1, dtype=torch.int64, device=gpu)
+    ok = lambda **kw: pa.paged_draft_attention(**{**dict(q=q, k_cache=k, v_cache=k, block_tables=t, context_lens=lens, tree_mask=m, scale=1.0), **kw})
+    ok()
+    for text, kw in (("tree_mask", dict(tree_mask=m.int())), ("tree_mask", dict(tree_mask=m[0])), ("tree_mask", dict(tree_mask=m.expand(2, 3, 2))),
+                     ("q ", dict(q=q[:, :2])), ("head_dim", dict(q=q[..., :32].contiguous())), ("block_tables", dict(block_tables=t[:1])),
+                     ("num_nodes", dict(num_nodes=lens[:1])), ("scale must be", dict(scale=0.0)), ("multiple of 32", dict(partition_size=8)),
+                     ("out must be", dict(out=q[:, :, :2])), ("cpu", dict(context_lens=lens.cpu())), ("multiple of num_kv_heads", dict(q=q[:, :, :3].contiguous())),
+                     ("fp8 cache", dict(k_cache=k.to(FP8), v_cache=k.to(FP8))), ("workspace", dict(partition_size=32, block_tables=t.repeat(1, 4), workspace=torch.empty(8, dtype=torch.uint8, device=gpu)))):
+        with pytest.raises(RuntimeError, match=text):
+            ok(**kw)
+    assert pa.paged_draft_attention(q[:0], k, k, t[:0], lens[:0], m[:1], 1.0).shape == (0, 3, 4, 64)
+
+
+# ---------------------------------------------------------------------------------------------- verification
+
+def make_logits(g, batch, nodes, vocab, dtype, spiky=True):
+    x = torch.randn(batch, nodes, vocab, generator=g) * 1.5
+    if spiky:
+        x.scatter_add_(2, torch.randint(0, vocab, (batch, nodes, 4), generator=g), torch.rand(batch, nodes, 4, generator=g) * 8)
+    return x.to(DT[dtype])
+
+
+def check_verify(pa, gpu, seed, batch, nodes, vocab, dtype, temperature, top_p, kind="tree", real=None, probs=None, spiky=True,
+                 change=None, shared=False, view=None):
+    rng = random.Random(seed)
+    g = torch.Generator().manual_seed(seed)
+    logits = make_logits(g, batch, nodes, vocab, dtype, spiky)
+    if change:
+        change(logits)
+    parents = [make_parents(kind, nodes, rng)] * batch if shared else [make_parents(kind, nodes, rng) for _ in range(batch)]
+    q = None
+    if probs:
+        q = torch.softmax(logits.float()[:, :-1] + 0.7 * torch.randn(batch, nodes - 1, vocab, generator=g), -1).to(DT[probs])
+        tokens = torch.cat([torch.zeros(batch, 1, dtype=torch.long),
+                            torch.multinomial(q.float().view(-1, vocab), 1, generator=g).view(batch, nodes - 1)], 1) if nodes > 1 \
+            else torch.zeros(batch, 1, dtype=torch.long)
+    else:
+        # likely tokens, some of them offered twice, some of them no tokens
+        tokens = torch.zeros(batch, nodes, dtype=torch.long)
+        for b in range(batch):
+            for c in range(1, nodes):
+                best = torch.topk(torch.nan_to_num(logits[b, parents[b][c]].float(), nan=-1e9), min(3, vocab)).indices
+                tokens[b, c] = int(best[rng.randrange(len(best))]) if rng.random() < 0.8 else rng.choice([0, vocab - 1, -1, vocab, 1 << 40])
+    u = torch.rand(batch, nodes, generator=g)
+    u[0, 0], u[-1, -1] = 0.0, 1.0 - 2.0 ** -24
+    dev = logits.to(gpu) if view is None else view(logits.to(gpu))
+    par = None if kind == "chain" and (probs or not shared) else torch.tensor(parents[0] if shared else parents, dtype=torch.int32, device=gpu)
+    got = pa.verify_drafts(dev, tokens.to(gpu), u.to(gpu), parents=par,
+                           num_nodes=None if real is None else torch.tensor(real, dtype=torch.int32, device=gpu),
+                           draft_probs=None if q is None else q.to(gpu), temperature=temperature, top_p=top_p)
+    emitted, counts, path = (t.tolist() for t in got)
+    for b in range(batch):
+        n = nodes if real is None else max(0, min(nodes, real[b]))
+        want, kept = so.verify(logits[b], tokens[b].tolist(), u[b].tolist(), parents[b], n, temperature, top_p, None if q is None else q[b].double())
+        pad = [-1] * (nodes - len(want))
+        assert counts[b] == len(want), (b, counts[b], want)
+        assert emitted[b] == want + pad and path[b] == kept + pad, (b, emitted[b], want)
+    return counts
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("temperature,top_p", [(0.0, 1.0), (1.0, 1.0), (0.7, 0.9), (1.3, 0.5), (0.05, 0.99), (1.0, 1e-9), (5.0, 0.999999)])
+def test_verify_trees(pa, gpu, dtype, temperature, top_p):
+    counts = check_verify(pa, gpu, 3, 24, 9, 331, dtype, temperature, top_p)
+    assert max(counts) > 1 and min(counts) >= 1
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("probs", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("temperature,top_p", [(1.0, 1.0), (0.8, 0.9), (0.0, 1.0)])
+def test_verify_chains_with_draft_probabilities(pa, gpu, dtype, probs, temperature, top_p):
+    counts = check_verify(pa, gpu, 4, 24, 5, 257, dtype, temperature, top_p, kind="chain", probs=probs)
+    assert max(counts) > 1
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 7, 8, 63, 64, 65, 1000, 2047, 2048, 2049, 5001, 16411])
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_verify_vocabularies(pa, gpu, vocab, dtype):
+    check_verify(pa, gpu, vocab, 5, 4, vocab, dtype, 1.0, 0.9, kind="deep")
+    check_verify(pa, gpu, vocab, 5, 3, vocab, dtype, 1.0, 1.0, kind="chain", probs="fp32")
+    check_verify(pa, gpu, vocab, 5, 4, vocab, dtype, 0.0, 1.0, kind="chain")
+
+
+@pytest.mark.parametrize("nodes", [1, 2, 64, 65, 200, 256])
+@pytest.mark.parametrize("kind", ["chain", "star", "tree"])
+def test_verify_tree_sizes(pa, gpu, nodes, kind):
+    check_verify(pa, gpu, nodes, 3, nodes, 90, "bf16", 1.0, 0.95, kind=kind, shared=kind == "star")
+
+
+def test_verify_short_and_padded_rows(pa, gpu):
+    counts = check_verify(pa, gpu, 8, 7, 6, 100, "fp16", 1.0, 0.9, real=[0, 1, 2, 6, 9, -3, 4])
+    assert counts[0] == counts[5] == 0 and counts[1] == 1
+    check_verify(pa, gpu, 8, 5, 6, 100, "fp16", 0.0, 1.0, real=[0, 1, 2, 6, 0])
+    check_verify(pa, gpu, 8, 5, 6, 100, "fp32", 1.0, 1.0, kind="chain", probs="fp32", real=[0, 1, 2, 6, 0])
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("temperature,top_p", [(1.0, 1.0), (0.7, 0.9), (0.0, 1.0)])
+def test_verify_rows_with_masked_and_extreme_logits(pa, gpu, dtype, temperature, top_p):
+    def extreme(x):
+        low = torch.finfo(x.dtype).min
+        x[0, :, 1::2] = -float("inf")
+        x[1, :, 5:] = low
+        x[2, :, ::3] = float("nan")
+        x[3] = 0.0                                            # all equal
+        x[3, :, ::2] = -0.0                                   # of both signs
+        x[4] = -x[4].abs() - 3                                # nothing positive
+        x[5, :, 7] = torch.finfo(x.dtype).max                 # one token takes everything
+        x[6] = low
+        x[7] = -float("inf")                                  # nothing at all
+        x[8] = float("nan")
+        x[9, :, :] = -float("inf")
+        x[9, :, 11] = 2.0                                     # a grammar that leaves one token
+    check_verify(pa, gpu, 13, 10, 5, 200, dtype, temperature, top_p, change=extreme)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("top_p", [0.9, 1.0])
+def test_verify_more_equal_logits_than_a_counter_holds(pa, gpu, dtype, top_p):
+    """65536 and more entries of one value in a row (a 16-bit counter wraps) next to rows without."""
+    def equal(x):
+        x[0, :, 100:66000] = -2.0
+        x[1, :, :] = 0.5
+        x[2, 0, 10:65546] = 0.0
+        x[2, 0, 65546:] = -0.0
+        x[3, :, 5:] = -float("inf")
+    check_verify(pa, gpu, 17, 5, 3, 70001, dtype, 1.0, top_p, kind="chain", change=equal, spiky=False)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("temperature,top_p", [(1.0, 1.0), (0.7, 0.9)])
+@pytest.mark.parametrize("spiky", [False, True])
+def test_verify_full_vocabulary(pa, gpu, dtype, temperature, top_p, spiky):
+    check_verify(pa, gpu, 19, 6, 4, 151936, dtype, temperature, top_p, spiky=spiky)
+    check_verify(pa, gpu, 20, 4, 3, 151936, dtype, temperature, top_p, spiky=spiky, kind="chain", probs="fp32")
+
+
+def test_verify_takes_views(pa, gpu):
+    check_verify(pa, gpu, 23, 3, 4, 101, "fp16", 1.0, 0.9, view=lambda x: torch.cat([x, x], 2)[:, :, :101])
+    check_verify(pa, gpu, 23, 3, 4, 101, "fp16", 1.0, 0.9, view=lambda x: torch.cat([x, x], 1)[:, :4])
+    check_verify(pa, gpu, 23, 3, 4, 101, "fp32", 1.0, 0.9, view=lambda x: x.transpose(1, 2).contiguous().transpose(1, 2))
+    check_verify(pa, gpu, 23, 3, 4, 101, "fp16", 0.0, 0.9, view=lambda x: x.transpose(0, 1).contiguous().transpose(0, 1))
+
+
+def test_verify_draws_its_own_uniforms(pa, gpu):
+    logits = torch.zeros(2048, 1, 4, device=gpu)
+    logits[..., 2] = math.log(3.0)                            # 1/6, 1/6, 1/2, 1/6
+    gen = torch.Generator(device=gpu).manual_seed(5)
+    tokens, counts, path = pa.verify_drafts(logits, torch.zeros(2048, 1, dtype=torch.long, device=gpu), generator=gen, temperature=1.0, top_p=1.0)
+    assert (counts == 1).all() and (path == 0).all()
+    share = torch.bincount(tokens.flatten(), minlength=4).double() / 2048
+    # five standard deviations of 2048 draws
+    assert (share.cpu() - torch.tensor([1 / 6, 1 / 6, 1 / 2, 1 / 6])).abs().max() < 5 * math.sqrt(0.25 / 2048)
+
+
+def test_verify_refusals(pa, gpu):
+    x = torch.zeros(2, 3, 8, device=gpu)
+    t = torch.zeros(2, 3, dtype=torch.long, device=gpu)
+    ok = lambda **kw: pa.verify_drafts(**{**dict(logits=x, draft_tokens=t), **kw})
+    ok()
+    p = torch.full((2, 2, 8), 0.125, device=gpu)
+    par = torch.tensor([-1, 0, 1], dtype=torch.int32, device=gpu)
+    for text, kw in (("logits", dict(logits=x[0])), ("draft_tokens", dict(draft_tokens=t.int())), ("draft_tokens", dict(draft_tokens=t[:1])),
+                     ("uniforms", dict(uniforms=torch.rand(2, 2, device=gpu))), ("uniforms", dict(uniforms=torch.rand(2, 3, device=gpu).double())),
+                     ("chains", dict(draft_probs=p, parents=par)), ("draft_probs", dict(draft_probs=p[:, :1])), ("parents", dict(parents=par[:2])),
+                     ("num_nodes", dict(num_nodes=par)), ("top_p", dict(top_p=0.0)), ("temperature", dict(temperature=1e9)),
+                     ("temperature", dict(temperature=float("nan"))), ("dtype", dict(logits=x.double())), ("cpu", dict(draft_tokens=t.cpu())),
+                     ("workspace", dict(workspace=torch.empty(8, dtype=torch.uint8, device=gpu)))):
+        with pytest.raises(RuntimeError, match=text):
+            ok(**kw)
+    assert pa.verify_drafts(x[:0], t[:0])[0].shape == (0, 3)
+
+
+# ---------------------------------------------------------------------------------------------- commit
+
+@pytest.mark.parametrize("cache", ["fp16", "fp32", "fp8"])
+@pytest.mark.parametrize("heads,dim,block", [(1, 64, 8), (2, 64, 16), (8, 128, 16), (40, 128, 5)])
+def test_commit_moves_the_kept_rows(pa, gpu, cache, heads, dim, block):
+    g = torch.Generator().manual_seed(heads)
+    rng = random.Random(heads)
+    nodes, layers = 40, 3
+    lens = [0, 3, 30, 77, 12, 5]
+    paths = [[0], [], [0, 1, 2, 3], [0] + sorted(rng.sample(range(1, nodes), 12)), [0, 39], [0] + sorted(rng.sample(range(1, nodes), 30))]
+    need = [(c + nodes + block - 1) // block for c in lens]
+    blocks = sum(need) + 2
+    order = torch.randperm(blocks, generator=g).tolist()
+    tables = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
+    at = 0
+    for b, k in enumerate(need):
+        tables[b, :k] = torch.tensor(order[at:at + k], dtype=torch.int32)
+        at += k
+    shape = (2, layers, blocks, block, heads, dim)
+    kv = torch.randint(0, 255, (*shape[:-1], dim * {"fp16": 2, "fp32": 4, "fp8": 1}[cache]), generator=g, dtype=torch.uint8).view(DT[cache])
+    scales = [torch.rand(layers, blocks, block, generator=g) for _ in range(2)] if cache == "fp8" else []
+    want, want_scales = kv.clone(), [s.clone() for s in scales]
+    raw = want.view(torch.uint8)
+    for b, path in enumerate(paths):
+        so.commit(raw, tables[b].tolist(), lens[b], path, block, want_scales)
+    path = torch.full((len(lens), nodes), -1, dtype=torch.int32)
+    for b, p in enumerate(paths):
+        path[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
+    counts = torch.tensor([len(p) for p in paths], dtype=torch.int32)
+    dev = kv.to(gpu)
+    dev_scales = [s.to(gpu) for s in scales]
+    lens_t = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    new = pa.commit_drafts(dev, tables.to(gpu), lens_t, path.to(gpu), counts.to(gpu), *dev_scales)
+    assert new.tolist() == [c + len(p) for c, p in zip(lens, paths)] and lens_t.tolist() == lens
+    assert torch.equal(dev.cpu().view(torch.uint8), raw)
+    for a, z in zip(dev_scales, want_scales):
+        assert torch.equal(a.cpu(), z)
+
+
+def test_commit_leaves_what_it_cannot_place(pa, gpu):
+    """Nodes that are none of the row's, positions outside the table or the pool, counts beyond the row."""
+    kv = torch.randn(2, 1, 4, 8, 1, 64, device=gpu)
+    before = kv.clone()
+    tables = torch.tensor([[0, -1], [1, 9], [2, 3]], dtype=torch.int32, device=gpu)
+    lens = torch.tensor([5, 6, 0], dtype=torch.int32, device=gpu)
+    path = torch.tensor([[0, 4, 5, -1], [0, 3, 99, 2], [0, 2, 1, 3]], dtype=torch.int32, device=gpu)
+    new = pa.commit_drafts(kv, tables, lens, path, torch.tensor([3, 4, 9], dtype=torch.int32, device=gpu))
+    assert new.tolist() == [8, 10, 4]
+    before[:, :, 2, 1] = before[:, :, 2, 2]                   # the only move that both ends of exist: row 2, node 2
+    assert torch.equal(kv, before)
+
+
+def test_commit_refusals(pa, gpu):
+    kv = torch.zeros(2, 1, 4, 8, 1, 64, device=gpu)
+    t = torch.zeros(2, 2, dtype=torch.int32, device=gpu)
+    lens = torch.tensor([1, 2], dtype=torch.int32, device=gpu)
+    path = torch.zeros(2, 3, dtype=torch.int32, device=gpu)
+    ok = lambda **kw: pa.commit_drafts(**{**dict(kv_cache=kv, block_tables=t, context_lens=lens, path=path, counts=lens), **kw})
+    ok()
+    for text, kw in (("kv_cache", dict(kv_cache=kv[0])), ("kv_cache", dict(kv_cache=kv[:, :, ::2])), ("path", dict(path=path[:1])),
+                     ("counts", dict(counts=lens[:1])), ("block_tables", dict(block_tables=t[:1])), ("cpu", dict(path=path.cpu())),
+                     ("fp8 pool", dict(kv_cache=kv.to(FP8)))):
+        with pytest.raises(RuntimeError, match=text):
+            ok(**kw)
+    assert pa.commit_drafts(kv, t[:0], lens[:0], path[:0], lens[:0]).shape == (0,)
