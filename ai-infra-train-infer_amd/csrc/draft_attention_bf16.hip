@@ -4,8 +4,8 @@
 
 namespace pa {
 
-int launch_draft_bf16(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st) {
-  return launch_draft<KV_BF16, CT_BF16>(p, head_dim, col_tiles, grid, st);
+int launch_draft_bf16(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st) {
+  return launch_draft<KV_BF16, CT_BF16>(p, head_dim, rows, grid, st);
 }
 
 }  // namespace pa

@@ -6,12 +6,13 @@
 // and a K/V row leaves HBM once for all of them: 2 G n FLOP per K/V element against 2 in a decode step, memory
 // bound up to R ~ 128 and bound by the matrix pipe and the exponentials beyond that.
 //
-//  * One workgroup per (batch row, KV head, tile of 16 C rows, partition); wave w of its 4 walks the 32-token
-//    tiles w, w + 4, ... of the partition on its own, without a barrier in the loop, and multiplies each with C
-//    16-row operands: the tile's fragments are read from LDS once for all C.
-//  * Loads, LDS layout and the two products are those of paged_decode_mfma_kernel.hpp: one tile of K and V in
-//    flight in registers (16 bytes per lane), written to the wave's own LDS, S^T = K . Q^T and O^T += V^T . P^T
-//    with 16x16x32 products, V^T through the LDS transpose read.
+//  * One workgroup of 4 waves per (batch row, KV head, tile of 16 ... 128 rows, partition).  Up to 16 rows
+//    (draft_narrow_kernel, memory bound): each wave walks its own 32-token tiles without a barrier, as a decode step's
+//    matrix kernel does.  More (draft_wide_kernel): the workgroup shares 64-token tiles and its waves split the rows, so
+//    that a K/V byte is fetched once per 128 rows.
+//  * Loads, LDS layout and the two products are those of paged_decode_mfma_kernel.hpp: tiles in flight in registers
+//    (16 bytes per lane), written to LDS, S^T = K . Q^T and O^T += V^T . P^T with 16x16x32 products, V^T through the
+//    LDS transpose read.
 //  * Queries keep their own bits (no scale folded in): 16-bit caches and queries of one type are multiplied as
 //    they are, everything else as fp16, and scale * log2(e) is applied to the fp32 score in the same fused
 //    multiply-add that subtracts the reference maximum.  What is rounded to 16 bits is the probability, in
@@ -20,10 +21,10 @@
 //    row's mask words.  A row that has seen nothing yet has reference -inf; one that sees nothing at all sums to
 //    zero and its output is zero.
 //  * NaN or infinity in the V of a node must not reach the nodes that do not see it, but a matrix product adds
-//    0 * NaN.  Tiles of drafted tokens are checked for such values on their way into LDS, and a tile that holds
-//    one goes through a key-by-key loop on the vector ALU that skips the zero probabilities.
-//  * The waves' partial results are merged through LDS, 16 rows at a time, and written to `out` or, as maximum,
-//    sum and normalised output, to the workspace.
+//    0 * NaN.  Tiles of drafted tokens enter LDS without such values; if there were any, the rows that do see them get
+//    them at the end (draft_wild).
+//  * Waves that took different tokens are merged through LDS; results go to `out` or, as maximum, sum and normalised
+//    output, to the workspace.
 #pragma once
 
 #include "paged_decode_mfma_kernel.hpp"
@@ -64,7 +65,7 @@ struct DraftParams {
   int table_width, bs_log2, num_blocks;
   int partition_size, max_partitions;
   int batch;
-  int row_tiles;                 // tiles of 16 C rows per KV head
+  int row_tiles;                 // workgroups' worth of rows per KV head
   float scale_log2e;
 };
 
@@ -103,10 +104,6 @@ __device__ __forceinline__ bool draft_unit(const DraftParams& p, int u, int lane
   return true;
 }
 
-__host__ __device__ constexpr int draft_lds_bytes(int C, int D) {
-  return kDraftWaves * decode_mfma_wave_bytes(1, D) + 2 * C * kMfmaHeads * kDraftWaves * 4;
-}
-
 // 8 source elements -> 8 elements of the products' type
 template <int KV, int CT>
 __device__ __forceinline__ mword4_t words_to_ct(const uint32_t* w) {
@@ -138,16 +135,325 @@ __device__ __forceinline__ float draft_unpack(uint32_t w, int half) {
   if constexpr (CT == CT_BF16) return bf16_bits_to_f32(h);
   else return f16_bits_to_f32(h);
 }
-// whether a word holds an infinity or NaN
+// Infinities and NaN become zeros; whether there were any.
 template <int CT>
-__device__ __forceinline__ bool draft_not_finite(uint32_t w) {
+__device__ __forceinline__ bool draft_tame(mword4_t& v) {
   constexpr uint32_t E = CT == CT_BF16 ? 0x7f80u : 0x7c00u;
-  return (w & E) == E || ((w >> 16) & E) == E;
+  bool wild = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const bool lo = (v[e] & E) == E, hi = (v[e] & (E << 16)) == (E << 16);
+    v[e] = (lo ? 0u : v[e] & 0xffffu) | (hi ? 0u : v[e] & 0xffff0000u);
+    wild = wild || lo || hi;
+  }
+  return wild;
 }
 
-// C 16-row operands per wave (see the head of this file)
+// LDS bytes of a 32-token tile of K, or of V
+__host__ __device__ constexpr int draft_half_bytes(int D) { return kMfmaTile * D * 2; }
+
+// What a wave keeps of its 16 C rows, and one step of them over 32 tokens in LDS.  Result layout of the products: lane
+// (col, kg) holds, for row 16 c + col, keys 4 kg .. + 3 of a 16-key half (scores) or dims 16 mt + 4 kg .. + 3 (output).
 template <int KV, int CT, int D, int C>
-__global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attention_kernel(const DraftParams p) {
+struct DraftRows {
+  static constexpr int KSTEPS = D / 32, MT = D / 16, ROWB = D * 2, CPR = D / 8;
+  mword4_t q[C][KSTEPS];         // Q^T as the B operand: dims 32 s + 8 kg .. + 7 of row 16 c + col
+  mfloat4_t o[C][MT];
+  float m_ref[C];                // reference maximum in log2 units, the same in a row's 4 lanes; -inf: nothing seen
+  float l_run[C];                // this lane's share of the row's sum
+  uint32_t k_off[KSTEPS], v_off[MT];
+  int col, kg;
+
+  __device__ __forceinline__ void init(int lane) {
+    col = lane & 15;
+    kg = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) k_off[s] = col * ROWB + (((4 * s + kg) ^ lds_swz<CPR>(col)) << 4);
+    // V^T through the transpose read: within a block of 16 lanes lane a supplies the address of 4 dims of key 4 kg + a / 4
+    const int key = 4 * kg + (col >> 2);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) v_off[mt] = key * ROWB + (((2 * mt + ((col & 3) >> 1)) ^ lds_swz<CPR>(key)) << 4) + (col & 1) * 8;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      m_ref[c] = -INFINITY;
+      l_run[c] = 0.0f;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) o[c][mt] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+  }
+
+  // at(c): element index of row 16 c + col's query
+  template <class At>
+  __device__ __forceinline__ void load_q(const void* ptr, int dtype, At&& at) {
+    // the dtype switch sits outside the loops: inside, it would put a branch and a wait between loads in flight
+    auto load = [&](auto dt_tag) __attribute__((always_inline)) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int64_t base = at(c) + 8 * kg;
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s) {
+          float x[8];
+          load8_as_f32(ptr, base + 32 * s, decltype(dt_tag)::value, x);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[c][s][e] = draft_pack<CT>(x[2 * e], x[2 * e + 1]);
+        }
+      }
+    };
+    if (dtype == PA_DTYPE_F16) load(std::integral_constant<int, PA_DTYPE_F16>{});
+    else if (dtype == PA_DTYPE_BF16) load(std::integral_constant<int, PA_DTYPE_BF16>{});
+    else load(std::integral_constant<int, PA_DTYPE_F32>{});
+  }
+
+  // k, v: the tile in LDS; iks, mvs: per token 1 / k_scale and the mantissa of 1 / v_scale (fp8).  visible(c): bit k =
+  // the row sees key k, asked for only in special tiles.
+  template <class Visible>
+  __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, const float* iks, const float* mvs_lds, float scale_log2e,
+                                       bool special, Visible&& visible) {
+    mfloat4_t s[C][2];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) s[c][kb] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int st = 0; st < KSTEPS; ++st)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const mword4_t a = *(const mword4_t*)(k + k_off[st] + kb * 16 * ROWB);
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[c][kb] = draft_mfma<CT>(a, q[c][st], s[c][kb]);
+      }
+    mfloat4_t mvs[2];
+    if constexpr (KV == KV_FP8) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        const float4 a = *(const float4*)&iks[16 * kb + 4 * kg];
+        const float4 m4 = *(const float4*)&mvs_lds[16 * kb + 4 * kg];
+        mvs[kb] = mfloat4_t{m4.x, m4.y, m4.z, m4.w};
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[c][kb] *= mfloat4_t{a.x, a.y, a.z, a.w};
+      }
+    }
+    if (special) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const uint32_t vis = visible(c) >> (4 * kg);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[c][kb][e] = (vis >> (16 * kb + e)) & 1u ? s[c][kb][e] : -INFINITY;
+      }
+    }
+    bool want = false;
+    float top[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      float mx = s[c][0][0];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[c][kb][e]);
+      top[c] = mx * scale_log2e;                           // scale > 0
+      want = want || top[c] > m_ref[c] + 8.0f;
+    }
+    // The reference follows a row's maximum only when that has outgrown it by 2^8: p <= 256 fits the 16-bit types,
+    // and the rescale of the accumulators almost never runs.
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(want) != 0, 0)) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float rmax = fmaxf(top[c], __shfl_xor(top[c], 16));
+        rmax = fmaxf(rmax, __shfl_xor(rmax, 32));
+        const bool grow = rmax > m_ref[c] + 8.0f;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m_ref[c] - rmax) : 1.0f;   // from -inf: 0 times nothing
+        m_ref[c] = grow ? rmax : m_ref[c];
+        l_run[c] *= alpha;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[c][mt][e] *= alpha;
+      }
+    }
+    // P^T as the B operand: contraction index 8 kg + e <-> key 4 kg + e (e < 4), 16 + 4 kg + e - 4
+    mword4_t pb[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float ref = m_ref[c] == -INFINITY ? 0.0f : m_ref[c];
+      float psum = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e], scale_log2e, -ref));
+          float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e + 1], scale_log2e, -ref));
+          psum += p0 + p1;
+          if constexpr (KV == KV_FP8) { p0 *= mvs[kb][e]; p1 *= mvs[kb][e + 1]; }
+          pb[c][2 * kb + e / 2] = draft_pack<CT>(p0, p1);
+        }
+      l_run[c] += psum;
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const uint8_t* at = v + v_off[mt];
+      const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)at);
+      const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(at + 16 * ROWB));
+      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+      const mword4_t a = {l2.x, l2.y, h2.x, h2.y};
+#pragma unroll
+      for (int c = 0; c < C; ++c) o[c][mt] = draft_mfma<CT>(a, pb[c], o[c][mt]);
+    }
+  }
+};
+
+// Which rows and tokens a workgroup takes.
+struct DraftWork {
+  int b, part, kvh, gq, row0;    // row0: first (node, head) row
+  int n, ctx, live, all;         // nodes drafted, committed tokens, rows of the workgroup with a node, rows of the launch
+  int begin, end;
+};
+
+// ROWS (node, head) rows per workgroup.  False: nothing to do (zeros for nodes that a row does not draft are written).
+template <int ROWS, int D>
+__device__ __forceinline__ bool draft_work(const DraftParams& p, DraftWork& w) {
+  const int inner = p.num_kv_heads * p.row_tiles;
+  const int in = blockIdx.x % inner, lane = threadIdx.x & 63;
+  w.b = blockIdx.x / inner;
+  w.part = 0;
+  if (p.max_partitions > 1) {
+    if (!draft_unit(p, blockIdx.x / inner, lane, w.b, w.part)) return false;
+    w.b = __builtin_amdgcn_readfirstlane(w.b);
+    w.part = __builtin_amdgcn_readfirstlane(w.part);
+  }
+  // KV heads fastest: the row tiles of a head are num_kv_heads workgroups apart, which with 8 heads puts them on one XCD
+  w.kvh = in % p.num_kv_heads;
+  w.gq = p.num_q_heads / p.num_kv_heads;
+  w.row0 = in / p.num_kv_heads * ROWS;
+  w.n = draft_nodes(p, w.b);
+  w.ctx = p.context_lens[w.b];
+  w.live = min(w.n * w.gq - w.row0, ROWS);
+  w.all = min(p.nodes * w.gq - w.row0, ROWS);
+  const int keys = w.ctx + w.n;
+  w.begin = 0;
+  w.end = keys;
+  if (p.max_partitions > 1) {
+    w.begin = w.part * p.partition_size;
+    w.end = w.part == p.max_partitions - 1 ? keys : min(w.begin + p.partition_size, keys);
+  }
+  return w.live > 0 && w.begin < w.end;
+}
+
+__device__ __forceinline__ int64_t draft_out_at(const DraftParams& p, const DraftWork& w, int r, int D) {
+  return ((int64_t)w.b * p.nodes + (w.row0 + r) / w.gq) * p.out_stride + (int64_t)(w.kvh * w.gq + (w.row0 + r) % w.gq) * D;
+}
+
+// zeros for the nodes that a row does not draft (a partitioned launch leaves them to the merge)
+template <int THREADS, int D>
+__device__ __forceinline__ void draft_zero_dead(const DraftParams& p, const DraftWork& w) {
+  if (p.max_partitions > 1) return;
+  for (int o = threadIdx.x + max(w.live, 0) * D; o < w.all * D; o += THREADS)
+    store_from_f32(p.out, draft_out_at(p, w, o / D, D) + o % D, p.q_dtype, 0.0f);
+}
+
+// The keys first .. first + 31 that row r sees, bit k = key first + k.
+__device__ __forceinline__ uint32_t draft_visible(const DraftParams& p, const DraftWork& w, int r, int first) {
+  const uint64_t* words = p.mask + w.b * p.mask_stride + (int64_t)((w.row0 + min(r, w.live - 1)) / w.gq) * p.words;
+  const int off = first - w.ctx;                           // the first key as a node; negative: committed keys come first
+  auto word = [&](int i) -> uint64_t { return i < p.words ? words[i] : 0ull; };
+  uint32_t bits = 0xffffffffu;
+  if (off >= 0) {
+    const int i = off >> 6, sh = off & 63;
+    uint64_t v = word(i) >> sh;
+    if (sh > 32) v |= word(i + 1) << (64 - sh);
+    bits = (uint32_t)v;
+  } else if (off > -32) {
+    bits = ((uint32_t)word(0) << -off) | ((1u << -off) - 1u);
+  }
+  const int left = w.end - first;                          // keys that exist
+  return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1u) : 0u;
+}
+
+// Writes one row's 4 dims of result, or of a partition's partial result.
+__device__ __forceinline__ void draft_store4(const DraftParams& p, const DraftWork& w, int r, int d, int D, const float (&x)[4]) {
+  if (p.max_partitions == 1) {
+    const int64_t at = draft_out_at(p, w, r, D) + d;
+    if (p.q_dtype == PA_DTYPE_F32) {
+      *(float4*)((float*)p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
+    } else if (p.q_dtype == PA_DTYPE_F16) {
+      *(uint2*)((uint16_t*)p.out + at) = make_uint2(draft_pack<CT_F16>(x[0], x[1]), draft_pack<CT_F16>(x[2], x[3]));
+    } else {
+      *(uint2*)((uint16_t*)p.out + at) = make_uint2(draft_pack<CT_BF16>(x[0], x[1]), draft_pack<CT_BF16>(x[2], x[3]));
+    }
+  } else {
+    const int rr = w.row0 + r;
+    const int64_t at = (((int64_t)w.b * p.nodes + rr / w.gq) * p.num_q_heads + w.kvh * w.gq + rr % w.gq) * p.max_partitions + w.part;
+    *(float4*)(p.ws_out + at * D + d) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+}
+__device__ __forceinline__ void draft_store_stats(const DraftParams& p, const DraftWork& w, int r, float top, float sum) {
+  const int rr = w.row0 + r;
+  const int64_t at = (((int64_t)w.b * p.nodes + rr / w.gq) * p.num_q_heads + w.kvh * w.gq + rr % w.gq) * p.max_partitions + w.part;
+  p.ws_max[at] = top;
+  p.ws_sum[at] = top == -INFINITY ? 0.0f : sum;
+}
+
+// The infinities and NaN that tiles of drafted tokens were multiplied without: a row that sees one gets the sum of those
+// it sees in that dim instead of its finite result.  Rare, so it reads V again from the cache, 8 dims of a row per thread.
+template <int KV, int CT, int D, int THREADS>
+__device__ __forceinline__ void draft_wild(const DraftParams& p, const DraftWork& w) {
+  constexpr int ES = KV == KV_FP8 ? 1 : 2;
+  __syncthreads();                   // the finite results are written
+  const int32_t* bt_row = p.block_tables + w.b * p.bt_stride;
+  const int first = max(w.begin, w.ctx - 63);              // no tile with a drafted token starts earlier
+  for (int item = threadIdx.x; item < w.live * (D / 8); item += THREADS) {
+    const int r = item / (D / 8), d = item % (D / 8) * 8;
+    float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    bool any = false;
+    for (int key = first; key < w.end; ++key) {
+      if (!(draft_visible(p, w, r, key) & 1u)) continue;
+      const int blk = min(key >> p.bs_log2, p.table_width - 1);
+      const int64_t phys = min(max(bt_row[blk], 0), p.num_blocks - 1);
+      const int64_t slot = (phys << p.bs_log2) + (key & ((1 << p.bs_log2) - 1));
+      const uint8_t* at = p.v_cache + ((slot * p.num_kv_heads + w.kvh) * D + d) * ES;
+      mword4_t v;
+      if constexpr (KV == KV_FP8) {
+        const uint32_t words[2] = {((const uint32_t*)at)[0], ((const uint32_t*)at)[1]};
+        const float pow2 = __uint_as_float(__float_as_uint(__builtin_amdgcn_rcpf(p.v_scale[slot])) & 0xff800000u);
+        v = __builtin_bit_cast(mword4_t, fp8_words_to_f16_pow2(words, pow2));
+      } else {
+        const mword4_t raw = *(const mword4_t*)at;
+        const uint32_t words[4] = {raw[0], raw[1], raw[2], raw[3]};
+        v = words_to_ct<KV, CT>(words);
+      }
+      mword4_t tame = v;
+      if (!draft_tame<CT>(tame)) continue;
+      any = true;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = draft_unpack<CT>(v[e / 2], e & 1);
+        if (!(fabsf(x) < INFINITY)) sum[e] += x;
+      }
+    }
+    if (!any) continue;
+    const int rr = w.row0 + r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (fabsf(sum[e]) < INFINITY) continue;              // nothing wild in this dim
+      if (p.max_partitions == 1) {
+        store_from_f32(p.out, draft_out_at(p, w, r, D) + d + e, p.q_dtype, sum[e]);
+      } else {
+        const int64_t at = (((int64_t)w.b * p.nodes + rr / w.gq) * p.num_q_heads + w.kvh * w.gq + rr % w.gq) * p.max_partitions + w.part;
+        p.ws_out[at * D + d + e] = sum[e];
+      }
+    }
+  }
+}
+
+// ---- up to 16 rows: every wave has its own tokens ----------------------------------------------------------------
+
+__host__ __device__ constexpr int draft_narrow_lds_bytes(int D) {
+  return kDraftWaves * decode_mfma_wave_bytes(1, D) + 2 * kMfmaHeads * kDraftWaves * 4 + 16;
+}
+
+template <int KV, int CT, int D>
+__global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const DraftParams p) {
   using G = Geo<KV, D, 1>;
   using TileT = MfmaTile<KV, D, 1>;
   constexpr int W = kDraftWaves;
@@ -156,86 +462,46 @@ __global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attent
   constexpr int RL = TileT::RL;              // row loads of 8 tokens per tile: 4
   constexpr int CPR = D / 8;
   constexpr int ROWB = D * 2;
-  constexpr int KSTEPS = D / 32;
   constexpr int MT = D / 16;
   constexpr int CPL = G::EPC / 8;
   constexpr bool LM = kLaneMajorTokens<KV>;
-  constexpr float NEG_INF = -INFINITY;
   constexpr int WAVEB = decode_mfma_wave_bytes(1, D);
 
   extern __shared__ __align__(16) uint8_t lds_raw[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint8_t* my_lds = lds_raw + wave * WAVEB;
-  float* my_scales = reinterpret_cast<float*>(my_lds + decode_mfma_tile_bytes(D));
+  float* my_scales = reinterpret_cast<float*>(my_lds + 2 * draft_half_bytes(D));
   float (*red)[NC * D] = reinterpret_cast<float (*)[NC * D]>(lds_raw);             // [W][16 x D], over the tiles
-  float (*sm)[W] = reinterpret_cast<float (*)[W]>(lds_raw + W * WAVEB);            // [16 C][W]
-  float (*sl)[W] = sm + C * NC;
+  float (*sm)[W] = reinterpret_cast<float (*)[W]>(lds_raw + W * WAVEB);            // [16][W]
+  float (*sl)[W] = sm + NC;
+  int* any_wild = reinterpret_cast<int*>(sl + NC);         // a drafted token's V holds infinities or NaN
 
   const int g = lane >> 3;
   const int j = lane & 7;
-  const int col = lane & 15;
-  const int kg = lane >> 4;
+  DraftWork w;
+  const bool some = draft_work<NC, D>(p, w);
+  draft_zero_dead<W * 64, D>(p, w);
+  if (!some) return;
+  DraftRows<KV, CT, D, 1> rows;
+  rows.init(lane);
+  const int col = rows.col, kg = rows.kg;
+  // rows without a node repeat the last one; they are never written
+  rows.load_q(p.q, p.q_dtype, [&](int c) {
+    const int r = w.row0 + min(col, w.live - 1);
+    return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
+  });
 
-  // ---- which rows and tokens --------------------------------------------------------------------------------
-  const int inner = p.num_kv_heads * p.row_tiles;
-  const int in = blockIdx.x % inner;
-  int b = blockIdx.x / inner, part = 0;
-  if (p.max_partitions > 1) {
-    if (!draft_unit(p, blockIdx.x / inner, lane, b, part)) return;
-    b = __builtin_amdgcn_readfirstlane(b);
-    part = __builtin_amdgcn_readfirstlane(part);
-  }
-  // KV heads fastest: the row tiles of a head are num_kv_heads workgroups apart, which with 8 heads puts them on one XCD
-  const int kvh = in % p.num_kv_heads;
-  const int gq = p.num_q_heads / p.num_kv_heads;
-  const int row0 = (in / p.num_kv_heads) * (NC * C);       // first (node, head) row of the workgroup
-  const int n = draft_nodes(p, b);
-  const int ctx = p.context_lens[b];
-  const int live = min(n * gq - row0, NC * C);             // rows of the workgroup that a node stands behind
-  const int all = min(p.nodes * gq - row0, NC * C);
-  const bool direct = p.max_partitions == 1;
-  auto out_at = [&](int r) { return ((int64_t)b * p.nodes + (row0 + r) / gq) * p.out_stride + (int64_t)(kvh * gq + (row0 + r) % gq) * D; };
-  if (direct)                                              // nodes the row does not draft
-    for (int o = threadIdx.x + max(live, 0) * D; o < all * D; o += W * 64) store_from_f32(p.out, out_at(o / D) + o % D, p.q_dtype, 0.0f);
-  if (live <= 0) return;
-  const int keys = ctx + n;
-  int begin = 0, end = keys;
-  if (!direct) {
-    begin = part * p.partition_size;
-    end = part == p.max_partitions - 1 ? keys : min(begin + p.partition_size, keys);
-  }
-  if (begin >= end) return;
+  if (threadIdx.x == 0) *any_wild = 0;
+  __syncthreads();
 
-  // ---- Q^T as the B operand: lane (col, kg) holds dims 32 s + 8 kg .. +7 of row 16 c + col ---------------------
-  mword4_t qreg[C][KSTEPS];
-  {
-    auto load_q = [&](auto dt_tag) __attribute__((always_inline)) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const int r = min(16 * c + col, live - 1);         // rows without a node repeat the last one; never written
-        const int64_t base = ((int64_t)b * p.nodes + (row0 + r) / gq) * p.q_stride + (int64_t)(kvh * gq + (row0 + r) % gq) * D + 8 * kg;
-#pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-          float x[8];
-          load8_as_f32(p.q, base + 32 * s, decltype(dt_tag)::value, x);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qreg[c][s][e] = draft_pack<CT>(x[2 * e], x[2 * e + 1]);
-        }
-      }
-    };
-    if (p.q_dtype == PA_DTYPE_F16) load_q(std::integral_constant<int, PA_DTYPE_F16>{});
-    else if (p.q_dtype == PA_DTYPE_BF16) load_q(std::integral_constant<int, PA_DTYPE_BF16>{});
-    else load_q(std::integral_constant<int, PA_DTYPE_F32>{});
-  }
-
-  // ---- loads ---------------------------------------------------------------------------------------------------
+  const int begin = w.begin, end = w.end;
   const int bs_mask = (1 << p.bs_log2) - 1;
   const uint32_t token_bytes = (uint32_t)(p.num_kv_heads * D * G::ES);
   const uint32_t block_bytes = token_bytes << p.bs_log2;
   auto token_of = [&](int r) { return LM ? g * 4 + r : r * 8 + g; };
-  const uint32_t lane_off = (uint32_t)(((LM ? 0 : g) * p.num_kv_heads + kvh) * D * G::ES + j * G::LB);
-  const int32_t* bt_row = p.block_tables + b * p.bt_stride;
+  const uint32_t lane_off = (uint32_t)(((LM ? 0 : g) * p.num_kv_heads + w.kvh) * D * G::ES + j * G::LB);
+  const int32_t* bt_row = p.block_tables + w.b * p.bt_stride;
   const int last_blk = min((end - 1) >> p.bs_log2, max(p.table_width - 1, 0));
   const int ntiles = (end - begin + TILE - 1) / TILE;
 
@@ -284,8 +550,8 @@ __global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attent
     }
   };
 
-  // ---- registers -> LDS; returns whether a drafted token's V (special tiles only) holds NaN or infinity ---------
-  auto write_tile = [&](TileT& t, int tile, bool special) __attribute__((always_inline)) -> bool {
+  // registers -> LDS
+  auto write_tile = [&](TileT& t, int tile, bool special) __attribute__((always_inline)) {
     bool wild = false;
 #pragma unroll
     for (int r = 0; r < RL; ++r) {
@@ -306,8 +572,7 @@ __global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attent
           else vf = words_to_ct<KV, CT>(&t.v[r][c * (G::LB / 4) + x * wpc]);
           if (special) {
             if (!valid) kf = vf = mword4_t{0, 0, 0, 0};     // past the end: scores masked, and 0 * V must stay 0
-#pragma unroll
-            for (int e = 0; e < 4; ++e) wild = wild || draft_not_finite<CT>(vf[e]);
+            wild = draft_tame<CT>(vf) || wild;
           }
           uint8_t* dst = my_lds + tk * ROWB + ((chunk ^ lds_swz<CPR>(tk)) << 4);
           *(mword4_t*)dst = kf;
@@ -327,175 +592,10 @@ __global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attent
       *(float4*)&my_scales[token_of(0)] = make_float4(ik[0], ik[1], ik[2], ik[3]);
       *(float4*)&my_scales[TILE + token_of(0)] = make_float4(mv[0], mv[1], mv[2], mv[3]);
     }
-    return wild;
+    if (special && wild) *any_wild = 1;
   };
 
-  // ---- LDS read addresses ----------------------------------------------------------------------------------------
-  const uint8_t* k_rd[KSTEPS];
-#pragma unroll
-  for (int s = 0; s < KSTEPS; ++s) k_rd[s] = my_lds + col * ROWB + (((4 * s + kg) ^ lds_swz<CPR>(col)) << 4);
-  const uint8_t* v_rd[MT];
-  {
-    const int key = 4 * kg + (col >> 2);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-      v_rd[mt] = my_lds + TILE * ROWB + key * ROWB + (((2 * mt + ((col & 3) >> 1)) ^ lds_swz<CPR>(key)) << 4) + (col & 1) * 8;
-  }
-
-  // The tile's keys that row 16 c + col sees, bit k = key k of the tile (special tiles only).
-  auto visible = [&](int c, int tile) __attribute__((always_inline)) -> uint32_t {
-    const int r = min(16 * c + col, live - 1);
-    const uint64_t* words = p.mask + b * p.mask_stride + (int64_t)((row0 + r) / gq) * p.words;
-    const int off = begin + tile * TILE - ctx;             // the tile's first key as a node; negative: committed keys come first
-    auto word = [&](int w) -> uint64_t { return w < p.words ? words[w] : 0ull; };
-    uint32_t bits = 0;
-    if (off >= 0) {
-      const int w = off >> 6, sh = off & 63;
-      uint64_t v = word(w) >> sh;
-      if (sh > 32) v |= word(w + 1) << (64 - sh);
-      bits = (uint32_t)v;
-    } else if (off > -32) {
-      bits = ((uint32_t)word(0) << -off) | ((1u << -off) - 1u);
-    } else {
-      bits = 0xffffffffu;
-    }
-    const int left = end - (begin + tile * TILE);          // keys of the tile that exist
-    return left < 32 ? bits & ((1u << left) - 1u) : bits;
-  };
-
-  float m_ref[C], l_run[C];      // reference maximum (log2 units, the same in a row's 4 lanes), this lane's share of the sum
-  mfloat4_t o[C][MT];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    m_ref[c] = NEG_INF;
-    l_run[c] = 0.0f;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) o[c][mt] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  auto compute = [&](int tile, bool special, bool wild) __attribute__((always_inline)) {
-    mfloat4_t s[C][2];
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) s[c][kb] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int st = 0; st < KSTEPS; ++st)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const mword4_t a = *(const mword4_t*)(k_rd[st] + kb * 16 * ROWB);
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[c][kb] = draft_mfma<CT>(a, qreg[c][st], s[c][kb]);
-      }
-    mfloat4_t mvs[2];
-    if constexpr (KV == KV_FP8) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const float4 a = *(const float4*)&my_scales[16 * kb + 4 * kg];
-        const float4 m4 = *(const float4*)&my_scales[TILE + 16 * kb + 4 * kg];
-        mvs[kb] = mfloat4_t{m4.x, m4.y, m4.z, m4.w};
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[c][kb] *= mfloat4_t{a.x, a.y, a.z, a.w};
-      }
-    }
-    if (special) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const uint32_t vis = visible(c, tile) >> (4 * kg);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[c][kb][e] = (vis >> (16 * kb + e)) & 1u ? s[c][kb][e] : NEG_INF;
-      }
-    }
-    bool want = false;
-    float top[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      float mx = s[c][0][0];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[c][kb][e]);
-      top[c] = mx * p.scale_log2e;                         // scale > 0
-      want = want || top[c] > m_ref[c] + 8.0f;
-    }
-    // The reference follows a row's maximum only when that has outgrown it by 2^8: p <= 256 fits the 16-bit types,
-    // and the rescale of the accumulators almost never runs.
-    if (__builtin_expect(__builtin_amdgcn_ballot_w64(want) != 0, 0)) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float rmax = fmaxf(top[c], __shfl_xor(top[c], 16));
-        rmax = fmaxf(rmax, __shfl_xor(rmax, 32));
-        const bool grow = rmax > m_ref[c] + 8.0f;
-        const float alpha = grow ? __builtin_amdgcn_exp2f(m_ref[c] - rmax) : 1.0f;   // from -inf: 0 times nothing
-        m_ref[c] = grow ? rmax : m_ref[c];
-        l_run[c] *= alpha;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[c][mt][e] *= alpha;
-      }
-    }
-    // ---- P^T as B operand: contraction index 8 kg + e <-> key 4 kg + e (e < 4), 16 + 4 kg + e - 4 ------------------
-    mword4_t pb[C];
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const float ref = m_ref[c] == NEG_INF ? 0.0f : m_ref[c];
-      float psum = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e], p.scale_log2e, -ref));
-          float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e + 1], p.scale_log2e, -ref));
-          psum += p0 + p1;
-          if constexpr (KV == KV_FP8) { p0 *= mvs[kb][e]; p1 *= mvs[kb][e + 1]; }
-          pb[c][2 * kb + e / 2] = draft_pack<CT>(p0, p1);
-        }
-      l_run[c] += psum;
-    }
-    if (__builtin_expect(wild, 0)) {
-      // a V row that must not be multiplied by the zeros of the rows that do not see it
-#pragma unroll 1
-      for (int key = 0; key < TILE; ++key) {
-        const int from = ((key & 15) >> 2) * 16 + col;     // the lane of this row that holds the key's probability
-        const int e = (key & 3) + 4 * (key >> 4);
-        float pk[C];
-        bool seen[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          uint32_t w = 0;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) w |= pb[c][x] & ((e >> 1) == x ? 0xffffffffu : 0u);
-          pk[c] = draft_unpack<CT>(__shfl(w, from), e & 1);
-          seen[c] = (visible(c, tile) >> key) & 1u;
-        }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint2 w = *(const uint2*)(my_lds + TILE * ROWB + key * ROWB + (((2 * mt + (kg >> 1)) ^ lds_swz<CPR>(key)) << 4) + (kg & 1) * 8);
-          const mfloat4_t v = {draft_unpack<CT>(w.x, 0), draft_unpack<CT>(w.x, 1), draft_unpack<CT>(w.y, 0), draft_unpack<CT>(w.y, 1)};
-#pragma unroll
-          for (int c = 0; c < C; ++c)
-#pragma unroll
-            for (int d = 0; d < 4; ++d) o[c][mt][d] = seen[c] ? fmaf(pk[c], v[d], o[c][mt][d]) : o[c][mt][d];
-        }
-      }
-      return;
-    }
-    // ---- O^T += V^T . P^T ---------------------------------------------------------------------------------------
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(v_rd[mt]));
-      const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(v_rd[mt] + 16 * ROWB));
-      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-      const mword4_t a = {l2.x, l2.y, h2.x, h2.y};
-#pragma unroll
-      for (int c = 0; c < C; ++c) o[c][mt] = draft_mfma<CT>(a, pb[c], o[c][mt]);
-    }
-  };
-
-  // ---- this wave's tiles: wave, wave + W, ... -------------------------------------------------------------------
+  // this wave's tiles: wave, wave + W, ...
   const int n_mine = ntiles > wave ? (ntiles - wave + W - 1) / W : 0;
   auto run_tiles = [&](auto stream_tag) __attribute__((always_inline)) {
     if (n_mine > 0) {
@@ -506,74 +606,261 @@ __global__ __launch_bounds__(kDraftWaves * 64, C == 1 ? 2 : 1) void draft_attent
       if (n_mine > 1) load_ids(wave + W, ids);
       for (int i = 0; i < n_mine; ++i) {
         const int tile = wave + i * W;
-        const int past = begin + (tile + 1) * TILE;
-        const bool special = past > ctx || past > end;     // drafted tokens or the end inside
+        const int first = begin + tile * TILE;
+        const bool special = first + TILE > w.ctx || first + TILE > end;     // drafted tokens or the end inside
         if (i + 2 < n_mine) load_ids(tile + 2 * W, ids_next);
-        const bool wild = write_tile(t, tile, special);
+        write_tile(t, tile, special);
         if (i + 1 < n_mine) issue_as(stream_tag, t, tile + W, ids);
-        compute(tile, special, special && __builtin_amdgcn_ballot_w64(wild) != 0);
+        rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, p.scale_log2e, special, [&](int) { return draft_visible(p, w, col, first); });
 #pragma unroll
         for (int x = 0; x < 4; ++x) ids[x] = ids_next[x];
       }
     }
   };
-  // non-temporal loads where nobody else reads the range: no second row tile, no neighbour with the same blocks
-  if (p.row_tiles == 1 && decode_range_is_private(bt_row, p.bt_stride, b, p.batch, min(begin >> p.bs_log2, last_blk)))
-    run_tiles(std::true_type{});
-  else
-    run_tiles(std::false_type{});
+  // non-temporal loads where no neighbour in the batch maps the same blocks
+  if (decode_range_is_private(bt_row, p.bt_stride, w.b, p.batch, min(begin >> p.bs_log2, last_blk))) run_tiles(std::true_type{});
+  else run_tiles(std::false_type{});
 
-  // ---- merge the waves ------------------------------------------------------------------------------------------
+  // merge the waves
+  if (kg == 0) sm[col][wave] = rows.m_ref[0];
+  __syncthreads();                   // the maxima are there; every wave is done with its tiles
+  float mx = sm[col][0];
 #pragma unroll
-  for (int c = 0; c < C; ++c)
-    if (kg == 0) sm[16 * c + col][wave] = m_ref[c];
+  for (int i = 1; i < W; ++i) mx = fmaxf(mx, sm[col][i]);
+  const float f = rows.m_ref[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rows.m_ref[0] - mx);
+  float lw = rows.l_run[0] * f;
+  lw += __shfl_xor(lw, 16);
+  lw += __shfl_xor(lw, 32);
+  if (kg == 0) sl[col][wave] = lw;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    __syncthreads();                 // the maxima are there; every wave is done with its tiles, or with the 16 rows before
-    float mx = sm[16 * c + col][0];
+  for (int mt = 0; mt < MT; ++mt)
+    *(float4*)&red[wave][col * D + 16 * mt + 4 * kg] = make_float4(rows.o[0][mt][0] * f, rows.o[0][mt][1] * f, rows.o[0][mt][2] * f, rows.o[0][mt][3] * f);
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < w.live * (D / 4); idx += W * 64) {
+    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f, top = -INFINITY;
 #pragma unroll
-    for (int i = 1; i < W; ++i) mx = fmaxf(mx, sm[16 * c + col][i]);
-    const float w = m_ref[c] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_ref[c] - mx);
-    float lw = l_run[c] * w;
-    lw += __shfl_xor(lw, 16);
-    lw += __shfl_xor(lw, 32);
-    if (kg == 0) sl[16 * c + col][wave] = lw;
+    for (int i = 0; i < W; ++i) {
+      const float4 v = *(const float4*)&red[i][r * D + d];
+      x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+      den += sl[r][i];
+      top = fmaxf(top, sm[r][i]);
+    }
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-      *(float4*)&red[wave][col * D + 16 * mt + 4 * kg] = make_float4(o[c][mt][0] * w, o[c][mt][1] * w, o[c][mt][2] * w, o[c][mt][3] * w);
-    __syncthreads();
-    const int rows = min(live - 16 * c, 16);
-    for (int idx = threadIdx.x; idx < rows * D; idx += W * 64) {
-      const int r = idx / D, d = idx % D;
-      float num = 0.0f, den = 0.0f, mo = NEG_INF;
+    for (int e = 0; e < 4; ++e) x[e] = top == -INFINITY ? 0.0f : x[e] / den;   // a row that saw no key: zero
+    draft_store4(p, w, r, d, D, x);
+    if (p.max_partitions > 1 && d == 0) draft_store_stats(p, w, r, top, den);
+  }
+  if (__builtin_expect(*any_wild, 0)) draft_wild<KV, CT, D, W * 64>(p, w);
+}
+
+// ---- more rows: the waves share the tokens -----------------------------------------------------------------------
+// 32 WR rows per workgroup.  A 64-token tile of K and V is fetched by the whole workgroup (the next tile's loads are in
+// flight in registers while this one is multiplied) and staged in LDS, double buffered, one barrier a tile.  WR = 4: wave
+// w takes rows 32 w .. of all 64 tokens; WR = 2, 1: wave w takes rows 32 (w / 2) .. (1: waves 0 and 1) of the tokens'
+// half w % 2, and the halves are merged at the end.
+
+constexpr int kWideTile = 64;
+
+__host__ __device__ constexpr int draft_wide_lds_bytes(int D) { return 2 * (4 * draft_half_bytes(D)) + 2 * 2 * kWideTile * 4 + 16; }
+
+template <int KV, int CT, int D, int WR>
+__global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const DraftParams p) {
+  constexpr int W = kDraftWaves, NT = W * 64;
+  constexpr int WK = WR == 4 ? 1 : 2;        // parts of a tile's tokens
+  constexpr int C = 2;                       // 16-row operands per wave
+  constexpr int ES = KV == KV_FP8 ? 1 : 2;
+  constexpr int LPR = D * ES / 16;           // threads per token row
+  constexpr int RPI = NT / LPR;              // rows per load instruction of the workgroup
+  constexpr int NIT = kWideTile / RPI;       // load instructions per tile (K and V each)
+  constexpr int CPT = 16 / ES / 8;           // 8-element chunks per load
+  constexpr int CPR = D / 8;
+  constexpr int ROWB = D * 2;
+  constexpr int MT = D / 16;
+  constexpr int HALF = draft_half_bytes(D);  // 32 tokens of K or V
+  static_assert(NIT >= 1, "a tile is at least one load per thread");
+
+  extern __shared__ __align__(16) uint8_t lds_raw[];
+  // stage: K (64 rows), V (64 rows); then per stage 1 / k_scale and the mantissa of 1 / v_scale; then any_wild
+  float* scales = reinterpret_cast<float*>(lds_raw + 2 * 4 * HALF);
+  int* any_wild = reinterpret_cast<int*>(scales + 2 * 2 * kWideTile);        // a drafted token's V holds infinities or NaN
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  DraftWork w;
+  const bool some = draft_work<32 * WR, D>(p, w);
+  draft_zero_dead<NT, D>(p, w);
+  if (!some) return;
+  const int wr = wave / WK, wk = wave % WK;
+  const bool active = wr < WR && 32 * wr < w.live;         // the wave has rows (it fetches tiles in any case)
+  const int row_w = 32 * wr;
+  DraftRows<KV, CT, D, C> rows;
+  rows.init(lane);
+  const int col = rows.col, kg = rows.kg;
+  rows.load_q(p.q, p.q_dtype, [&](int c) {
+    const int r = w.row0 + min(row_w + 16 * c + col, w.live - 1);
+    return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
+  });
+
+  const int begin = w.begin, end = w.end;
+  const int bs_mask = (1 << p.bs_log2) - 1;
+  const uint32_t token_bytes = (uint32_t)(p.num_kv_heads * D * ES);
+  const uint32_t block_bytes = token_bytes << p.bs_log2;
+  const int32_t* bt_row = p.block_tables + w.b * p.bt_stride;
+  const int last_blk = min((end - 1) >> p.bs_log2, max(p.table_width - 1, 0));
+  const int ntiles = (end - begin + kWideTile - 1) / kWideTile;
+  const int lrow = tid / LPR;                // this thread's row of a load instruction
+  const uint32_t lane_off = (uint32_t)(w.kvh * D * ES + (tid % LPR) * 16);
+
+  mword4_t st_k[NIT], st_v[NIT];             // the next tile, as loaded
+  float st_ks[NIT], st_vs[NIT];
+  int ids[NIT];                              // its table entries, fetched a tile ahead of the loads that need them
+  auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        num += red[i][idx];
-        den += sl[16 * c + r][i];
-        mo = fmaxf(mo, sm[16 * c + r][i]);
+    for (int i = 0; i < NIT; ++i) ids[i] = bt_row[min((begin + tile * kWideTile + i * RPI + lrow) >> p.bs_log2, last_blk)];
+  };
+  auto issue = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      const uint32_t phys = (uint32_t)min(max(ids[i], 0), p.num_blocks - 1);
+      const uint32_t off = (uint32_t)((begin + tile * kWideTile + i * RPI + lrow) & bs_mask);
+      const uint64_t base = (uint64_t)phys * block_bytes + off * token_bytes + lane_off;
+      st_k[i] = *(const mword4_t*)(p.k_cache + base);
+      st_v[i] = *(const mword4_t*)(p.v_cache + base);
+      if constexpr (KV == KV_FP8) {
+        const uint64_t slot = ((uint64_t)phys << p.bs_log2) + off;
+        st_ks[i] = p.k_scale[slot];
+        st_vs[i] = p.v_scale[slot];
       }
-      const float res = mo == NEG_INF ? 0.0f : num / den;  // a row that saw no key: zero
-      if (direct) {
-        store_from_f32(p.out, out_at(16 * c + r) + d, p.q_dtype, res);
-      } else {
-        const int rr = row0 + 16 * c + r;
-        const int64_t at = (((int64_t)b * p.nodes + rr / gq) * p.num_q_heads + kvh * gq + rr % gq) * p.max_partitions + part;
-        p.ws_out[at * D + d] = res;
-        if (d == 0) {
-          p.ws_max[at] = mo;
-          p.ws_sum[at] = mo == NEG_INF ? 0.0f : den;
+    }
+  };
+  auto commit = [&](int tile) __attribute__((always_inline)) {
+    const int buf = tile & 1;
+    uint8_t* kt = lds_raw + buf * 4 * HALF;
+    const int past = begin + (tile + 1) * kWideTile;
+    const bool special = past > w.ctx || past > end;
+    bool wild = false;
+#pragma unroll
+    for (int i = 0; i < NIT; ++i) {
+      const int r = i * RPI + lrow;
+      const bool valid = begin + tile * kWideTile + r < end;
+      float v_pow2 = 1.0f;
+      if constexpr (KV == KV_FP8) v_pow2 = __uint_as_float(__float_as_uint(__builtin_amdgcn_rcpf(st_vs[i])) & 0xff800000u);
+#pragma unroll
+      for (int x = 0; x < CPT; ++x) {
+        const int chunk = (tid % LPR) * CPT + x;
+        const uint32_t kw[4] = {st_k[i][0], st_k[i][1], st_k[i][2], st_k[i][3]};
+        const uint32_t vw[4] = {st_v[i][0], st_v[i][1], st_v[i][2], st_v[i][3]};
+        mword4_t kf = words_to_ct<KV, CT>(kw + 2 * x);
+        mword4_t vf;
+        if constexpr (KV == KV_FP8) vf = __builtin_bit_cast(mword4_t, fp8_words_to_f16_pow2(vw + 2 * x, v_pow2));
+        else vf = words_to_ct<KV, CT>(vw);
+        if (special) {
+          if (!valid) kf = vf = mword4_t{0, 0, 0, 0};       // past the end: scores masked, and 0 * V must stay 0
+          wild = draft_tame<CT>(vf) || wild;
+        }
+        uint8_t* dst = kt + r * ROWB + ((chunk ^ lds_swz<CPR>(r)) << 4);
+        *(mword4_t*)dst = kf;
+        *(mword4_t*)(dst + 2 * HALF) = vf;
+      }
+      if constexpr (KV == KV_FP8) {
+        if (tid % LPR == 0) {
+          const uint32_t bits = __float_as_uint(__builtin_amdgcn_rcpf(st_vs[i]));
+          scales[buf * 2 * kWideTile + r] = valid ? __builtin_amdgcn_rcpf(st_ks[i]) : 0.0f;
+          scales[buf * 2 * kWideTile + kWideTile + r] = valid ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 0.0f;
         }
       }
     }
+    if (special && wild) *any_wild = 1;
+  };
+
+  if (tid == 0) *any_wild = 0;
+  load_ids(0);
+  issue(0);
+  load_ids(1);
+  __syncthreads();
+  commit(0);
+  if (ntiles > 1) issue(1);
+  load_ids(2);
+  __syncthreads();
+  for (int tile = 0; tile < ntiles; ++tile) {
+    const uint8_t* kt = lds_raw + (tile & 1) * 4 * HALF;
+    const float* sc = scales + (tile & 1) * 2 * kWideTile;
+    if (active) {
+#pragma unroll 1                     // one copy of the step: two, interleaved by the scheduler, do not fit the registers
+      for (int h = 0; h < 2 / WK; ++h) {
+        const int half = WK == 2 ? wk : h;
+        const int first = begin + tile * kWideTile + half * 32;
+        if (first < end) {
+          const bool special = first + 32 > w.ctx || first + 32 > end;       // drafted tokens or the end inside
+          rows.step(kt + half * HALF, kt + (2 + half) * HALF, sc + half * 32, sc + kWideTile + half * 32, p.scale_log2e, special,
+                    [&](int c) { return draft_visible(p, w, row_w + 16 * c + col, first); });
+        }
+      }
+    }
+    if (tile + 1 < ntiles) {
+      commit(tile + 1);              // the other stage: its last readers passed the barrier before this tile
+      if (tile + 2 < ntiles) issue(tile + 2);
+      load_ids(tile + 3);
+    }
+    __syncthreads();
   }
+
+  // ---- merge the halves, write --------------------------------------------------------------------------------------
+  float sum[C], top[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    sum[c] = rows.l_run[c];
+    sum[c] += __shfl_xor(sum[c], 16);
+    sum[c] += __shfl_xor(sum[c], 32);
+    top[c] = rows.m_ref[c];
+  }
+  if constexpr (WK == 2) {
+    float* other = reinterpret_cast<float*>(lds_raw) + wr * (C * 16 * (D + 4));        // [32][D + 4]: output, maximum, sum
+    if (active && wk == 1) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        float* at = other + (16 * c + col) * (D + 4);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) *(mfloat4_t*)(at + 16 * mt + 4 * kg) = rows.o[c][mt];
+        if (kg == 0) { at[D] = top[c]; at[D + 1] = sum[c]; }
+      }
+    }
+    __syncthreads();
+    if (active && wk == 0) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const float* at = other + (16 * c + col) * (D + 4);
+        const float t1 = at[D], mx = fmaxf(top[c], t1);
+        const float f0 = top[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[c] - mx);
+        const float f1 = t1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t1 - mx);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) rows.o[c][mt] = rows.o[c][mt] * f0 + *(const mfloat4_t*)(at + 16 * mt + 4 * kg) * f1;
+        sum[c] = sum[c] * f0 + at[D + 1] * f1;
+        top[c] = mx;
+      }
+    }
+  }
+  if (active && wk == 0) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int r = row_w + 16 * c + col;
+      if (r >= w.live) continue;
+      const float inv = top[c] == -INFINITY ? 0.0f : 1.0f / sum[c];          // a row that saw no key: zero
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const float x[4] = {rows.o[c][mt][0] * inv, rows.o[c][mt][1] * inv, rows.o[c][mt][2] * inv, rows.o[c][mt][3] * inv};
+        draft_store4(p, w, r, 16 * mt + 4 * kg, D, x);
+      }
+      if (p.max_partitions > 1 && kg == 0) draft_store_stats(p, w, r, top[c], sum[c]);
+    }
+  }
+  if (__builtin_expect(*any_wild, 0)) draft_wild<KV, CT, D, NT>(p, w);
 }
 
-template <int KV, int CT, int D, int C>
-int launch_draft_shape(const DraftParams& p, unsigned grid, hipStream_t st) {
-  auto kern = draft_attention_kernel<KV, CT, D, C>;
-  constexpr int lds = draft_lds_bytes(C, D);
-  // the attribute belongs to the kernel on one device: once per instantiation and device
-  static std::atomic<bool> attr_set[64];
+using DraftKernel = void (*)(DraftParams);
+
+// `attr_set`: one flag per device, the kernel's own (the LDS limit belongs to the kernel on one device)
+inline int launch_draft_kernel(DraftKernel kern, int lds, std::atomic<bool>* attr_set, const DraftParams& p, unsigned grid, hipStream_t st) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return fail(PA_ERR_LAUNCH, "pa_draft_attention: cannot tell the current device");
   if (!attr_set[dev].load(std::memory_order_acquire)) {
@@ -585,16 +872,32 @@ int launch_draft_shape(const DraftParams& p, unsigned grid, hipStream_t st) {
   return PA_OK;
 }
 
-template <int KV, int CT>
-int launch_draft(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st) {
-  if (head_dim == 128)
-    return col_tiles == 1 ? launch_draft_shape<KV, CT, 128, 1>(p, grid, st) : launch_draft_shape<KV, CT, 128, 2>(p, grid, st);
-  return col_tiles == 1 ? launch_draft_shape<KV, CT, 64, 1>(p, grid, st) : launch_draft_shape<KV, CT, 64, 2>(p, grid, st);
+template <int KV, int CT, int D, int ROWS>
+int launch_draft_rows(const DraftParams& p, unsigned grid, hipStream_t st) {
+  static std::atomic<bool> attr_set[64];
+  if constexpr (ROWS == 16) return launch_draft_kernel(draft_narrow_kernel<KV, CT, D>, draft_narrow_lds_bytes(D), attr_set, p, grid, st);
+  else return launch_draft_kernel(draft_wide_kernel<KV, CT, D, ROWS / 32>, draft_wide_lds_bytes(D), attr_set, p, grid, st);
 }
 
-int launch_draft_f16(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st);
-int launch_draft_bf16(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st);
-int launch_draft_bf16_as_f16(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st);
-int launch_draft_fp8(const DraftParams& p, int head_dim, int col_tiles, unsigned grid, hipStream_t st);
+template <int KV, int CT, int D>
+int launch_draft_dim(const DraftParams& p, int rows, unsigned grid, hipStream_t st) {
+  switch (rows) {
+    case 16: return launch_draft_rows<KV, CT, D, 16>(p, grid, st);
+    case 32: return launch_draft_rows<KV, CT, D, 32>(p, grid, st);
+    case 64: return launch_draft_rows<KV, CT, D, 64>(p, grid, st);
+    default: return launch_draft_rows<KV, CT, D, 128>(p, grid, st);
+  }
+}
+
+// rows: (node, head) rows per workgroup, 16, 32, 64 or 128
+template <int KV, int CT>
+int launch_draft(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st) {
+  return head_dim == 128 ? launch_draft_dim<KV, CT, 128>(p, rows, grid, st) : launch_draft_dim<KV, CT, 64>(p, rows, grid, st);
+}
+
+int launch_draft_f16(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st);
+int launch_draft_bf16(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st);
+int launch_draft_bf16_as_f16(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st);
+int launch_draft_fp8(const DraftParams& p, int head_dim, int rows, unsigned grid, hipStream_t st);
 
 }  // namespace pa

@@ -115,7 +115,7 @@ _MAX_PARTITIONS = 64
 @functools.lru_cache(maxsize=4096)
 def _choose_draft_partition(batch, rows, num_kv_heads, max_keys, compute_units):
     """(partition_size, max_partitions): the tokens of a row are cut until about two workgroups per CU exist."""
-    tiles = -(-rows // (16 if rows <= 16 else 32))
+    tiles = -(-rows // (16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128))
     units = max(1, batch * num_kv_heads * tiles)
     parts = min(-(-2 * compute_units // units), _MAX_PARTITIONS, -(-max_keys // _MIN_PARTITION))
     if parts <= 1:

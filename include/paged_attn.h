@@ -564,8 +564,8 @@ int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int6
  *   max_partitions       1: one pass; > 1: the tokens of a row (committed and drafted) are cut every
  *                        partition_size tokens as in pa_decode, and a second launch merges
  *   workspace            >= pa_draft_workspace_bytes(...) bytes, 256-byte aligned, when max_partitions > 1
- *   col_tiles            16-row tiles of (node, query head) rows of one KV head that a wave multiplies with a
- *                        K/V tile: 1, 2, or 0 = the launch's own choice; the result does not depend on it
+ *   rows_per_workgroup   (node, query head) rows of one KV head that a workgroup serves from one pass over K and
+ *                        V: 16, 32, 64, 128, or 0 = the launch's own choice; never changes what is computed
  * Cache, tables, scales and sizes as for pa_decode.  16-bit caches and queries of one type are multiplied as they
  * are, everything else as fp16; accumulation and softmax statistics are fp32.
  */
@@ -578,7 +578,7 @@ int pa_draft_attention(const void* q, int q_dtype, int64_t q_stride, const void*
                        int64_t out_stride, int64_t batch, int64_t nodes, int64_t num_q_heads,
                        int64_t num_kv_heads, int64_t head_dim, int64_t block_size, int64_t num_blocks,
                        float scale, int64_t partition_size, int64_t max_partitions, void* workspace,
-                       int64_t workspace_bytes, int col_tiles, void* stream);
+                       int64_t workspace_bytes, int rows_per_workgroup, void* stream);
 
 #ifdef __cplusplus
 }
