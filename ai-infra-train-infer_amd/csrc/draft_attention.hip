@@ -6,64 +6,71 @@ namespace pa {
 // out = sum_p w_p out_p / sum_p w_p with w_p = sum_p * 2^(max_p - max) over the partitions of a (node, query head) row that
 // hold tokens; a row that saw nothing in any of them is zero, and so is a node that the row does not draft.
 // D / 4 threads read one partial result 16 bytes each; `slots` of them side by side take the row's partitions in turn, and
-// 256 / (slots x D / 4) rows share a workgroup: with few partitions a row needs few threads, with many they are read at once
-// (5 nodes x 16 heads, 17 partitions: 11.9 us with one wave a row that walked them).
+// 256 / (slots x D / 4) rows share a workgroup: with few partitions a row needs few threads, with many they are read at once.
+// Bound by latency: the maxima and sums, the context length that says how many of them count, and the first partial results
+// are all asked for before anything is waited for (whatever lies behind the row's last partition is loaded and not used),
+// and the weights meet in LDS.
 constexpr int kDraftMergeThreads = 256;
+constexpr int kDraftMergeAhead = 4;       // partial results per thread in flight
 
 template <int D>
-__global__ __launch_bounds__(kDraftMergeThreads) void draft_merge_kernel(const DraftParams p, const int slots, const int64_t rows) {
-  __shared__ float4 s_acc[kDraftMergeThreads];
-  __shared__ float s_top[kDraftMergeThreads], s_den[kDraftMergeThreads];
+__global__ __launch_bounds__(kDraftMergeThreads) void draft_merge_kernel(const DraftParams p, const int slots, const int rows) {
+  extern __shared__ float lds[];            // rows of the workgroup x (2 x max_partitions), then 256 x 4 floats
   constexpr int LPP = D / 4;
-  const int tid = threadIdx.x, ld = tid % LPP, slot = tid / LPP % slots;
-  const int group = slots * LPP;
-  const int64_t row = (int64_t)blockIdx.x * (kDraftMergeThreads / group) + tid / group;
-  const int head = row % p.num_q_heads;
-  const int64_t bn = row / p.num_q_heads;
+  const int np_max = p.max_partitions;
+  const int group = slots * LPP, per_wg = kDraftMergeThreads / group;
+  const int tid = threadIdx.x, tg = tid % group, ld = tid % LPP, slot = tg / LPP, lr = tid / group;
+  const int row = min((int)blockIdx.x * per_wg + lr, rows - 1);     // a surplus group repeats the last row and does not write
+  const bool writes = (int)blockIdx.x * per_wg + lr < rows;
+  const int head = row % p.num_q_heads, bn = row / p.num_q_heads;
   const int node = bn % p.nodes, b = bn / p.nodes;
-  float top = -INFINITY, den = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const bool live = row < rows && node < draft_nodes(p, b);
-  if (live) {
-    const int np = min((draft_keys(p, b) + p.partition_size - 1) / p.partition_size, p.max_partitions);
-    const int64_t at = row * p.max_partitions;
-#pragma unroll 2
-    for (int q = slot; q < np; q += slots) {
-      const float pt = p.ws_max[at + q], ps = p.ws_sum[at + q];
-      const float4 v = *(const float4*)(p.ws_out + (at + q) * D + 4 * ld);
-      const float next = fmaxf(top, pt);
-      const float a = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top - next);
-      const float w = pt == -INFINITY ? 0.0f : ps * __builtin_amdgcn_exp2f(pt - next);
-      top = next;
-      den = den * a + w;
-      if (a == 0.0f) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      else { acc.x *= a; acc.y *= a; acc.z *= a; acc.w *= a; }
-      if (w != 0.0f) { acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w; }
-    }
+  const int64_t at = (int64_t)row * np_max;
+  float* s_max = lds + lr * 2 * np_max;
+  float* s_w = s_max + np_max;
+  float4 ahead[kDraftMergeAhead];
+#pragma unroll
+  for (int k = 0; k < kDraftMergeAhead; ++k) {
+    const int q = slot + k * slots;
+    ahead[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (q < np_max) ahead[k] = *(const float4*)(p.ws_out + (at + q) * D + 4 * ld);
   }
-  s_acc[tid] = acc;
-  s_top[tid] = top;
-  s_den[tid] = den;
+  const bool live = node < draft_nodes(p, b);
+  const int np = live ? min((draft_keys(p, b) + p.partition_size - 1) / p.partition_size, np_max) : 0;
+  for (int q = tg; q < np_max; q += group) {
+    const float m = p.ws_max[at + q], w = p.ws_sum[at + q];
+    s_max[q] = q < np ? m : -INFINITY;
+    s_w[q] = w;
+  }
   __syncthreads();
-  if (slot != 0 || row >= rows) return;
-  float all = top;
-  for (int i = 1; i < slots; ++i) all = fmaxf(all, s_top[tid + i * LPP]);
-  float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total = 0.0f;
-  if (all != -INFINITY) {
-    for (int i = 0; i < slots; ++i) {
-      const float t = s_top[tid + i * LPP];
-      if (t == -INFINITY) continue;
-      const float w = __builtin_amdgcn_exp2f(t - all);
-      const float4 v = s_acc[tid + i * LPP];
-      total += w * s_den[tid + i * LPP];
-      x[0] += w * v.x; x[1] += w * v.y; x[2] += w * v.z; x[3] += w * v.w;
-    }
+  float top = -INFINITY;
+  for (int q = 0; q < np; ++q) top = fmaxf(top, s_max[q]);
+  for (int q = tg; q < np; q += group) s_w[q] = s_max[q] == -INFINITY ? 0.0f : s_w[q] * __builtin_amdgcn_exp2f(s_max[q] - top);
+  __syncthreads();
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](int q, const float4& v) __attribute__((always_inline)) {
+    const float w = q < np ? s_w[q] : 0.0f;
+    if (w != 0.0f) { acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w; }
+  };
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] /= total;
+  for (int k = 0; k < kDraftMergeAhead; ++k) add(slot + k * slots, ahead[k]);
+#pragma unroll 4
+  for (int q = slot + kDraftMergeAhead * slots; q < np; q += slots) add(q, *(const float4*)(p.ws_out + (at + q) * D + 4 * ld));
+  float4* s_acc = (float4*)(lds + (per_wg * 2 * np_max + 3) / 4 * 4);
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (slot != 0 || !writes) return;
+  float den = 0.0f;
+  for (int q = 0; q < np; ++q) den += s_w[q];
+  for (int i = 1; i < slots; ++i) {
+    const float4 v = s_acc[tid + i * LPP];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
-  const int64_t o = bn * p.out_stride + (int64_t)head * D + 4 * ld;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) store_from_f32(p.out, o + e, p.q_dtype, x[e]);
+  const float inv = top == -INFINITY ? 0.0f : 1.0f / den;
+  const int64_t o = (int64_t)bn * p.out_stride + (int64_t)head * D + 4 * ld;
+  const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (p.q_dtype == PA_DTYPE_F32) *(float4*)((float*)p.out + o) = make_float4(x[0], x[1], x[2], x[3]);
+  else if (p.q_dtype == PA_DTYPE_F16) *(uint2*)((uint16_t*)p.out + o) = make_uint2(draft_pack<CT_F16>(x[0], x[1]), draft_pack<CT_F16>(x[2], x[3]));
+  else *(uint2*)((uint16_t*)p.out + o) = make_uint2(draft_pack<CT_BF16>(x[0], x[1]), draft_pack<CT_BF16>(x[2], x[3]));
 }
 
 static int64_t draft_rows_bytes(int64_t rows) { return (rows * 4 + 255) / 256 * 256; }
@@ -118,6 +125,11 @@ extern "C" int pa_draft_attention(const void* q, int q_dtype, int64_t q_stride, 
   if (tile != 0 && tile != 16 && tile != 32 && tile != 64 && tile != 128)
     DRAFT_FAIL(PA_ERR_BAD_ARG, "rows_per_workgroup must be 0, 16, 32, 64 or 128");
   if (max_partitions < 1) DRAFT_FAIL(PA_ERR_BAD_ARG, "max_partitions must be positive");
+  if (max_partitions > 1024) DRAFT_FAIL(PA_ERR_UNSUPPORTED, "more than 1024 partitions");
+  if (batch * nodes * num_q_heads > 0x7fffffff) DRAFT_FAIL(PA_ERR_UNSUPPORTED, "too many rows for one launch");
+  // results are written 8 (f32: 16) bytes at a time
+  if ((reinterpret_cast<uintptr_t>(out) & (q_dtype == PA_DTYPE_F32 ? 15u : 7u)) != 0 || out_stride % 4 != 0)
+    DRAFT_FAIL(PA_ERR_BAD_ARG, "out rows must be 8-byte aligned (f32: 16)");
   if (max_partitions > 1) {
     if (partition_size <= 0 || partition_size % 32 != 0 || partition_size > 0x7fffff00)
       DRAFT_FAIL(PA_ERR_UNSUPPORTED, "partition_size must be a positive multiple of 32");
@@ -178,11 +190,10 @@ extern "C" int pa_draft_attention(const void* q, int q_dtype, int64_t q_stride, 
     int slots = 1;
     while (slots < most && slots * 2 <= max_partitions) slots *= 2;
     const int64_t per_wg = kDraftMergeThreads / (slots * (head_dim / 4));
-    const int64_t merge_wgs = (out_rows + per_wg - 1) / per_wg;
-    if (merge_wgs > 0x7fffffff) return fail(PA_ERR_UNSUPPORTED, "pa_draft_attention: too many workgroups for one launch");
-    const dim3 grid((unsigned)merge_wgs);
-    if (head_dim == 128) hipLaunchKernelGGL(draft_merge_kernel<128>, grid, dim3(kDraftMergeThreads), 0, st, p, slots, out_rows);
-    else hipLaunchKernelGGL(draft_merge_kernel<64>, grid, dim3(kDraftMergeThreads), 0, st, p, slots, out_rows);
+    const dim3 grid((unsigned)((out_rows + per_wg - 1) / per_wg));
+    const size_t lds = (size_t)((per_wg * 2 * max_partitions + 3) / 4 * 4 + kDraftMergeThreads * 4) * 4;
+    if (head_dim == 128) hipLaunchKernelGGL(draft_merge_kernel<128>, grid, dim3(kDraftMergeThreads), lds, st, p, slots, (int)out_rows);
+    else hipLaunchKernelGGL(draft_merge_kernel<64>, grid, dim3(kDraftMergeThreads), lds, st, p, slots, (int)out_rows);
   }
   return check_launch("pa_draft_attention");
 }

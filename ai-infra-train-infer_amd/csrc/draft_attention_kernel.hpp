@@ -6,7 +6,7 @@
 // and a K/V row leaves HBM once for all of them: 2 G n FLOP per K/V element against 2 in a decode step, memory
 // bound up to R ~ 128 and bound by the matrix pipe and the exponentials beyond that.
 //
-//  * One workgroup of 4 waves per (batch row, KV head, tile of 16 ... 128 rows, partition).  Up to 16 rows
+//  * One workgroup of 4 or 8 waves per (batch row, KV head, tile of 16 ... 128 rows, partition).  Up to 16 rows
 //    (draft_narrow_kernel, memory bound): each wave walks its own 32-token tiles without a barrier, as a decode step's
 //    matrix kernel does.  More (draft_wide_kernel): the workgroup shares 64-token tiles and its waves split the rows, so
 //    that a K/V byte is fetched once per 128 rows.
@@ -38,8 +38,6 @@ enum : int { CT_F16 = 0, CT_BF16 = 1 };   // what the products multiply
 typedef __bf16 mbf8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 mbf2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t mword4_t __attribute__((ext_vector_type(4)));
-
-constexpr int kDraftWaves = 4;
 
 struct DraftParams {
   const void* q;
@@ -154,7 +152,8 @@ __host__ __device__ constexpr int draft_half_bytes(int D) { return kMfmaTile * D
 
 // What a wave keeps of its 16 C rows, and one step of them over 32 tokens in LDS.  Result layout of the products: lane
 // (col, kg) holds, for row 16 c + col, keys 4 kg .. + 3 of a 16-key half (scores) or dims 16 mt + 4 kg .. + 3 (output).
-template <int KV, int CT, int D, int C>
+// AHEAD: a step asks for V's fragments before its softmax (32 registers more at head_dim 128).
+template <int KV, int CT, int D, int C, bool AHEAD = true>
 struct DraftRows {
   static constexpr int KSTEPS = D / 32, MT = D / 16, ROWB = D * 2, CPR = D / 8;
   mword4_t q[C][KSTEPS];         // Q^T as the B operand: dims 32 s + 8 kg .. + 7 of row 16 c + col
@@ -214,14 +213,33 @@ struct DraftRows {
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) s[c][kb] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    // All of K's fragments are requested before the first product, all of V's before the softmax: left to the scheduler a
+    // product waits for the read issued just before it.
+    mword4_t ka[KSTEPS][2];
 #pragma unroll
     for (int st = 0; st < KSTEPS; ++st)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const mword4_t a = *(const mword4_t*)(k + k_off[st] + kb * 16 * ROWB);
+      for (int kb = 0; kb < 2; ++kb) ka[st][kb] = *(const mword4_t*)(k + k_off[st] + kb * 16 * ROWB);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int c = 0; c < C; ++c) s[c][kb] = draft_mfma<CT>(a, q[c][st], s[c][kb]);
-      }
+    for (int st = 0; st < KSTEPS; ++st)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int c = 0; c < C; ++c) s[c][kb] = draft_mfma<CT>(ka[st][kb], q[c][st], s[c][kb]);
+    auto load_v = [&](int mt) __attribute__((always_inline)) {
+      const uint8_t* at = v + v_off[mt];
+      const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)at);
+      const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(at + 16 * ROWB));
+      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+      return mword4_t{l2.x, l2.y, h2.x, h2.y};
+    };
+    mword4_t va[AHEAD ? MT : 1];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) va[mt] = load_v(mt);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     mfloat4_t mvs[2];
     if constexpr (KV == KV_FP8) {
 #pragma unroll
@@ -292,11 +310,7 @@ struct DraftRows {
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const uint8_t* at = v + v_off[mt];
-      const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)at);
-      const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(at + 16 * ROWB));
-      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-      const mword4_t a = {l2.x, l2.y, h2.x, h2.y};
+      const mword4_t a = AHEAD ? va[AHEAD ? mt : 0] : load_v(mt);
 #pragma unroll
       for (int c = 0; c < C; ++c) o[c][mt] = draft_mfma<CT>(a, pb[c], o[c][mt]);
     }
@@ -446,17 +460,21 @@ __device__ __forceinline__ void draft_wild(const DraftParams& p, const DraftWork
   }
 }
 
-// ---- up to 16 rows: every wave has its own tokens ----------------------------------------------------------------
+// ---- up to 32 rows: every wave has its own tokens ----------------------------------------------------------------
 
-__host__ __device__ constexpr int draft_narrow_lds_bytes(int D) {
-  return kDraftWaves * decode_mfma_wave_bytes(1, D) + 2 * kMfmaHeads * kDraftWaves * 4 + 16;
+// C 16-row operands, 1 or 2.  (8 waves a workgroup in launches of fewer workgroups than CUs changed nothing: a lone
+// workgroup is bound by what its CU can pull, about 70 GB/s, and more partitions put more CUs to work.)
+constexpr int kDraftWaves = 4;
+
+__host__ __device__ constexpr int draft_narrow_lds_bytes(int D, int C) {
+  return kDraftWaves * decode_mfma_wave_bytes(1, D) + 2 * C * kMfmaHeads * kDraftWaves * 4 + 16;
 }
 
-template <int KV, int CT, int D>
+template <int KV, int CT, int D, int C>
 __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const DraftParams p) {
+  constexpr int W = kDraftWaves;
   using G = Geo<KV, D, 1>;
   using TileT = MfmaTile<KV, D, 1>;
-  constexpr int W = kDraftWaves;
   constexpr int TILE = kMfmaTile;
   constexpr int NC = kMfmaHeads;
   constexpr int RL = TileT::RL;              // row loads of 8 tokens per tile: 4
@@ -472,23 +490,23 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint8_t* my_lds = lds_raw + wave * WAVEB;
   float* my_scales = reinterpret_cast<float*>(my_lds + 2 * draft_half_bytes(D));
-  float (*red)[NC * D] = reinterpret_cast<float (*)[NC * D]>(lds_raw);             // [W][16 x D], over the tiles
-  float (*sm)[W] = reinterpret_cast<float (*)[W]>(lds_raw + W * WAVEB);            // [16][W]
-  float (*sl)[W] = sm + NC;
-  int* any_wild = reinterpret_cast<int*>(sl + NC);         // a drafted token's V holds infinities or NaN
+  float (*red)[NC * D] = reinterpret_cast<float (*)[NC * D]>(lds_raw);             // [W][16 x D], over the tiles, one operand at a time
+  float (*sm)[W] = reinterpret_cast<float (*)[W]>(lds_raw + W * WAVEB);            // [16 C][W]
+  float (*sl)[W] = sm + C * NC;
+  int* any_wild = reinterpret_cast<int*>(sl + C * NC);         // a drafted token's V holds infinities or NaN
 
   const int g = lane >> 3;
   const int j = lane & 7;
   DraftWork w;
-  const bool some = draft_work<NC, D>(p, w);
+  const bool some = draft_work<C * NC, D>(p, w);
   draft_zero_dead<W * 64, D>(p, w);
   if (!some) return;
-  DraftRows<KV, CT, D, 1> rows;
+  DraftRows<KV, CT, D, C, C == 1> rows;       // with two operands V's fragments ahead of time would not fit 256 registers
   rows.init(lane);
   const int col = rows.col, kg = rows.kg;
   // rows without a node repeat the last one; they are never written
   rows.load_q(p.q, p.q_dtype, [&](int c) {
-    const int r = w.row0 + min(col, w.live - 1);
+    const int r = w.row0 + min(16 * c + col, w.live - 1);
     return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
   });
 
@@ -611,7 +629,7 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
         if (i + 2 < n_mine) load_ids(tile + 2 * W, ids_next);
         write_tile(t, tile, special);
         if (i + 1 < n_mine) issue_as(stream_tag, t, tile + W, ids);
-        rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, p.scale_log2e, special, [&](int) { return draft_visible(p, w, col, first); });
+        rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, p.scale_log2e, special, [&](int c) { return draft_visible(p, w, 16 * c + col, first); });
 #pragma unroll
         for (int x = 0; x < 4; ++x) ids[x] = ids_next[x];
       }
@@ -622,75 +640,86 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
   else run_tiles(std::false_type{});
 
   // merge the waves
-  if (kg == 0) sm[col][wave] = rows.m_ref[0];
-  __syncthreads();                   // the maxima are there; every wave is done with its tiles
-  float mx = sm[col][0];
 #pragma unroll
-  for (int i = 1; i < W; ++i) mx = fmaxf(mx, sm[col][i]);
-  const float f = rows.m_ref[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rows.m_ref[0] - mx);
-  float lw = rows.l_run[0] * f;
-  lw += __shfl_xor(lw, 16);
-  lw += __shfl_xor(lw, 32);
-  if (kg == 0) sl[col][wave] = lw;
+  for (int c = 0; c < C; ++c)
+    if (kg == 0) sm[16 * c + col][wave] = rows.m_ref[c];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-    *(float4*)&red[wave][col * D + 16 * mt + 4 * kg] = make_float4(rows.o[0][mt][0] * f, rows.o[0][mt][1] * f, rows.o[0][mt][2] * f, rows.o[0][mt][3] * f);
-  __syncthreads();
-  for (int idx = threadIdx.x; idx < w.live * (D / 4); idx += W * 64) {
-    const int r = idx / (D / 4), d = idx % (D / 4) * 4;
-    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f, top = -INFINITY;
+  for (int c = 0; c < C; ++c) {
+    __syncthreads();                 // the maxima are there; every wave is done with its tiles, or with the operand before
+    float mx = sm[16 * c + col][0];
 #pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const float4 v = *(const float4*)&red[i][r * D + d];
-      x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
-      den += sl[r][i];
-      top = fmaxf(top, sm[r][i]);
+    for (int i = 1; i < W; ++i) mx = fmaxf(mx, sm[16 * c + col][i]);
+    const float f = rows.m_ref[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rows.m_ref[c] - mx);
+    float lw = rows.l_run[c] * f;
+    lw += __shfl_xor(lw, 16);
+    lw += __shfl_xor(lw, 32);
+    if (kg == 0) sl[16 * c + col][wave] = lw;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) *(mfloat4_t*)&red[wave][col * D + 16 * mt + 4 * kg] = rows.o[c][mt] * f;
+    __syncthreads();
+    const int some_rows = min(w.live - 16 * c, 16);
+    for (int idx = threadIdx.x; idx < some_rows * (D / 4); idx += W * 64) {
+      const int r = idx / (D / 4), d = idx % (D / 4) * 4;
+      float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, den = 0.0f, top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        const float4 v = *(const float4*)&red[i][r * D + d];
+        x[0] += v.x; x[1] += v.y; x[2] += v.z; x[3] += v.w;
+        den += sl[16 * c + r][i];
+        top = fmaxf(top, sm[16 * c + r][i]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = top == -INFINITY ? 0.0f : x[e] / den;   // a row that saw no key: zero
+      draft_store4(p, w, 16 * c + r, d, D, x);
+      if (p.max_partitions > 1 && d == 0) draft_store_stats(p, w, 16 * c + r, top, den);
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = top == -INFINITY ? 0.0f : x[e] / den;   // a row that saw no key: zero
-    draft_store4(p, w, r, d, D, x);
-    if (p.max_partitions > 1 && d == 0) draft_store_stats(p, w, r, top, den);
   }
   if (__builtin_expect(*any_wild, 0)) draft_wild<KV, CT, D, W * 64>(p, w);
 }
 
 // ---- more rows: the waves share the tokens -----------------------------------------------------------------------
-// 32 WR rows per workgroup.  A 64-token tile of K and V is fetched by the whole workgroup (the next tile's loads are in
-// flight in registers while this one is multiplied) and staged in LDS, double buffered, one barrier a tile.  WR = 4: wave
-// w takes rows 32 w .. of all 64 tokens; WR = 2, 1: wave w takes rows 32 (w / 2) .. (1: waves 0 and 1) of the tokens'
-// half w % 2, and the halves are merged at the end.
+// 32 WR rows per workgroup.  A 64-token tile of K and V is fetched by the whole workgroup and staged in LDS, double
+// buffered, one barrier a tile; the next DEPTH tiles' loads are in flight in registers meanwhile.  Wave (wr, wk) takes
+// rows 32 wr .. + 31 of the tile's half wk (WR = 1 with 4 waves: waves 2 and 3 only fetch), and the halves are merged at
+// the end.  8 waves for 128 rows: a CU then holds one workgroup with two waves per SIMD, whose products and exponentials
+// overlap, and 64 KiB of loads in flight (4 waves taking all 64 tokens each, one tile ahead: 32 rows of 64 nodes x 4096
+// tokens took 146 us, of which the loads by themselves were 104).
 
 constexpr int kWideTile = 64;
-
-__host__ __device__ constexpr int draft_wide_lds_bytes(int D) { return 2 * (4 * draft_half_bytes(D)) + 2 * 2 * kWideTile * 4 + 16; }
+__host__ __device__ constexpr int draft_wide_waves(int WR) { return WR == 4 ? 8 : 4; }
+__host__ __device__ constexpr int draft_wide_stage_bytes(int D, int WR) {
+  const int tiles = 2 * kWideTile * D * 4, merge = WR * 32 * (D + 4) * 4;
+  return tiles > merge ? tiles : merge;
+}
+__host__ __device__ constexpr int draft_wide_lds_bytes(int D, int WR) { return draft_wide_stage_bytes(D, WR) + 2 * 2 * kWideTile * 4 + 16; }
 
 template <int KV, int CT, int D, int WR>
-__global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const DraftParams p) {
-  constexpr int W = kDraftWaves, NT = W * 64;
-  constexpr int WK = WR == 4 ? 1 : 2;        // parts of a tile's tokens
+__global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kernel(const DraftParams p) {
+  constexpr int W = draft_wide_waves(WR), NT = W * 64;
+  constexpr int TK = kWideTile;
+  constexpr int DEPTH = W == 8 ? 2 : 1;
   constexpr int C = 2;                       // 16-row operands per wave
   constexpr int ES = KV == KV_FP8 ? 1 : 2;
   constexpr int LPR = D * ES / 16;           // threads per token row
-  constexpr int RPI = NT / LPR;              // rows per load instruction of the workgroup
-  constexpr int NIT = kWideTile / RPI;       // load instructions per tile (K and V each)
+  constexpr int RPI = NT / LPR < TK ? NT / LPR : TK;     // rows per load instruction of the workgroup
+  constexpr int NIT = TK / RPI;       // load instructions per tile (K and V each)
   constexpr int CPT = 16 / ES / 8;           // 8-element chunks per load
   constexpr int CPR = D / 8;
   constexpr int ROWB = D * 2;
   constexpr int MT = D / 16;
-  constexpr int HALF = draft_half_bytes(D);  // 32 tokens of K or V
-  static_assert(NIT >= 1, "a tile is at least one load per thread");
+  constexpr int TILEB = TK * ROWB;           // the tile's K or V
 
   extern __shared__ __align__(16) uint8_t lds_raw[];
-  // stage: K (64 rows), V (64 rows); then per stage 1 / k_scale and the mantissa of 1 / v_scale; then any_wild
-  float* scales = reinterpret_cast<float*>(lds_raw + 2 * 4 * HALF);
-  int* any_wild = reinterpret_cast<int*>(scales + 2 * 2 * kWideTile);        // a drafted token's V holds infinities or NaN
+  // stage: K, V; then per stage 1 / k_scale and the mantissa of 1 / v_scale; then any_wild
+  float* scales = reinterpret_cast<float*>(lds_raw + draft_wide_stage_bytes(D, WR));
+  int* any_wild = reinterpret_cast<int*>(scales + 2 * 2 * TK);        // a drafted token's V holds infinities or NaN
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   DraftWork w;
   const bool some = draft_work<32 * WR, D>(p, w);
   draft_zero_dead<NT, D>(p, w);
   if (!some) return;
-  const int wr = wave / WK, wk = wave % WK;
+  const int wr = wave >> 1, wk = wave & 1;
   const bool active = wr < WR && 32 * wr < w.live;         // the wave has rows (it fetches tiles in any case)
   const int row_w = 32 * wr;
   DraftRows<KV, CT, D, C> rows;
@@ -707,49 +736,71 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const D
   const uint32_t block_bytes = token_bytes << p.bs_log2;
   const int32_t* bt_row = p.block_tables + w.b * p.bt_stride;
   const int last_blk = min((end - 1) >> p.bs_log2, max(p.table_width - 1, 0));
-  const int ntiles = (end - begin + kWideTile - 1) / kWideTile;
+  const int ntiles = (end - begin + TK - 1) / TK;
   const int lrow = tid / LPR;                // this thread's row of a load instruction
+  const bool fetches = LPR * TK >= NT || lrow < TK;      // narrow fp8 rows need only part of the workgroup
   const uint32_t lane_off = (uint32_t)(w.kvh * D * ES + (tid % LPR) * 16);
+  // non-temporal loads where nobody else reads the range: no second row tile, no neighbour with the same blocks
+  const bool stream = p.row_tiles == 1 && decode_range_is_private(bt_row, p.bt_stride, w.b, p.batch, min(begin >> p.bs_log2, last_blk));
 
-  mword4_t st_k[NIT], st_v[NIT];             // the next tile, as loaded
-  float st_ks[NIT], st_vs[NIT];
-  int ids[NIT];                              // its table entries, fetched a tile ahead of the loads that need them
+  struct Stage {                             // a tile as loaded
+    mword4_t k[NIT], v[NIT];
+    float ks[NIT], vs[NIT];
+  };
+  Stage st[DEPTH];
+  int ids[NIT];                              // table entries of the next tile to ask for, fetched a tile ahead of its loads
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < NIT; ++i) ids[i] = bt_row[min((begin + tile * kWideTile + i * RPI + lrow) >> p.bs_log2, last_blk)];
+    for (int i = 0; i < NIT; ++i) ids[i] = bt_row[min((begin + tile * TK + i * RPI + lrow) >> p.bs_log2, last_blk)];
   };
-  auto issue = [&](int tile) __attribute__((always_inline)) {
+  // The next tile's table entries are asked for before this tile's data: loads return in order, and a wait for entries asked
+  // for behind the data would be a wait for the data.
+  auto issue = [&](Stage& t, int tile) __attribute__((always_inline)) {
+    int now[NIT];
 #pragma unroll
-    for (int i = 0; i < NIT; ++i) {
-      const uint32_t phys = (uint32_t)min(max(ids[i], 0), p.num_blocks - 1);
-      const uint32_t off = (uint32_t)((begin + tile * kWideTile + i * RPI + lrow) & bs_mask);
-      const uint64_t base = (uint64_t)phys * block_bytes + off * token_bytes + lane_off;
-      st_k[i] = *(const mword4_t*)(p.k_cache + base);
-      st_v[i] = *(const mword4_t*)(p.v_cache + base);
-      if constexpr (KV == KV_FP8) {
-        const uint64_t slot = ((uint64_t)phys << p.bs_log2) + off;
-        st_ks[i] = p.k_scale[slot];
-        st_vs[i] = p.v_scale[slot];
+    for (int i = 0; i < NIT; ++i) now[i] = ids[i];
+    load_ids(tile + 1);
+    if (tile < ntiles && fetches) {
+#pragma unroll
+      for (int i = 0; i < NIT; ++i) {
+        const uint32_t phys = (uint32_t)min(max(now[i], 0), p.num_blocks - 1);
+        const uint32_t off = (uint32_t)((begin + tile * TK + i * RPI + lrow) & bs_mask);
+        const uint64_t base = (uint64_t)phys * block_bytes + off * token_bytes + lane_off;
+        const mword4_t* kp = (const mword4_t*)(p.k_cache + base);
+        const mword4_t* vp = (const mword4_t*)(p.v_cache + base);
+        if (stream) {
+          t.k[i] = __builtin_nontemporal_load(kp);
+          t.v[i] = __builtin_nontemporal_load(vp);
+        } else {
+          t.k[i] = *kp;
+          t.v[i] = *vp;
+        }
+        if constexpr (KV == KV_FP8) {
+          const uint64_t slot = ((uint64_t)phys << p.bs_log2) + off;
+          t.ks[i] = p.k_scale[slot];
+          t.vs[i] = p.v_scale[slot];
+        }
       }
     }
   };
-  auto commit = [&](int tile) __attribute__((always_inline)) {
+  auto commit = [&](Stage& t, int tile) __attribute__((always_inline)) {
+    if (tile >= ntiles || !fetches) return;
     const int buf = tile & 1;
-    uint8_t* kt = lds_raw + buf * 4 * HALF;
-    const int past = begin + (tile + 1) * kWideTile;
+    uint8_t* kt = lds_raw + buf * 2 * TILEB;
+    const int past = begin + (tile + 1) * TK;
     const bool special = past > w.ctx || past > end;
     bool wild = false;
 #pragma unroll
     for (int i = 0; i < NIT; ++i) {
       const int r = i * RPI + lrow;
-      const bool valid = begin + tile * kWideTile + r < end;
+      const bool valid = begin + tile * TK + r < end;
       float v_pow2 = 1.0f;
-      if constexpr (KV == KV_FP8) v_pow2 = __uint_as_float(__float_as_uint(__builtin_amdgcn_rcpf(st_vs[i])) & 0xff800000u);
+      if constexpr (KV == KV_FP8) v_pow2 = __uint_as_float(__float_as_uint(__builtin_amdgcn_rcpf(t.vs[i])) & 0xff800000u);
 #pragma unroll
       for (int x = 0; x < CPT; ++x) {
         const int chunk = (tid % LPR) * CPT + x;
-        const uint32_t kw[4] = {st_k[i][0], st_k[i][1], st_k[i][2], st_k[i][3]};
-        const uint32_t vw[4] = {st_v[i][0], st_v[i][1], st_v[i][2], st_v[i][3]};
+        const uint32_t kw[4] = {t.k[i][0], t.k[i][1], t.k[i][2], t.k[i][3]};
+        const uint32_t vw[4] = {t.v[i][0], t.v[i][1], t.v[i][2], t.v[i][3]};
         mword4_t kf = words_to_ct<KV, CT>(kw + 2 * x);
         mword4_t vf;
         if constexpr (KV == KV_FP8) vf = __builtin_bit_cast(mword4_t, fp8_words_to_f16_pow2(vw + 2 * x, v_pow2));
@@ -760,49 +811,50 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const D
         }
         uint8_t* dst = kt + r * ROWB + ((chunk ^ lds_swz<CPR>(r)) << 4);
         *(mword4_t*)dst = kf;
-        *(mword4_t*)(dst + 2 * HALF) = vf;
+        *(mword4_t*)(dst + TILEB) = vf;
       }
       if constexpr (KV == KV_FP8) {
         if (tid % LPR == 0) {
-          const uint32_t bits = __float_as_uint(__builtin_amdgcn_rcpf(st_vs[i]));
-          scales[buf * 2 * kWideTile + r] = valid ? __builtin_amdgcn_rcpf(st_ks[i]) : 0.0f;
-          scales[buf * 2 * kWideTile + kWideTile + r] = valid ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 0.0f;
+          const uint32_t bits = __float_as_uint(__builtin_amdgcn_rcpf(t.vs[i]));
+          scales[buf * 2 * TK + r] = valid ? __builtin_amdgcn_rcpf(t.ks[i]) : 0.0f;
+          scales[buf * 2 * TK + TK + r] = valid ? __uint_as_float((bits & 0x007fffffu) | 0x3f800000u) : 0.0f;
         }
       }
     }
     if (special && wild) *any_wild = 1;
   };
+  auto compute = [&](int tile) __attribute__((always_inline)) {
+    if (!active) return;
+    const uint8_t* kt = lds_raw + (tile & 1) * 2 * TILEB;
+    const float* sc = scales + (tile & 1) * 2 * TK;
+    const int at = wk * (TK / 2), first = begin + tile * TK + at;
+    if (first >= end) return;
+    const bool special = first + 32 > w.ctx || first + 32 > end;       // drafted tokens or the end inside
+    rows.step(kt + at * ROWB, kt + TILEB + at * ROWB, sc + at, sc + TK + at, p.scale_log2e, special,
+              [&](int c) { return draft_visible(p, w, row_w + 16 * c + col, first); });
+  };
 
   if (tid == 0) *any_wild = 0;
   load_ids(0);
-  issue(0);
-  load_ids(1);
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) issue(st[d], d);
   __syncthreads();
-  commit(0);
-  if (ntiles > 1) issue(1);
-  load_ids(2);
+  commit(st[0], 0);
+  issue(st[0], DEPTH);
   __syncthreads();
-  for (int tile = 0; tile < ntiles; ++tile) {
-    const uint8_t* kt = lds_raw + (tile & 1) * 4 * HALF;
-    const float* sc = scales + (tile & 1) * 2 * kWideTile;
-    if (active) {
-#pragma unroll 1                     // one copy of the step: two, interleaved by the scheduler, do not fit the registers
-      for (int h = 0; h < 2 / WK; ++h) {
-        const int half = WK == 2 ? wk : h;
-        const int first = begin + tile * kWideTile + half * 32;
-        if (first < end) {
-          const bool special = first + 32 > w.ctx || first + 32 > end;       // drafted tokens or the end inside
-          rows.step(kt + half * HALF, kt + (2 + half) * HALF, sc + half * 32, sc + kWideTile + half * 32, p.scale_log2e, special,
-                    [&](int c) { return draft_visible(p, w, row_w + 16 * c + col, first); });
-        }
+  // before step `tile`: its tile is in LDS, tiles + 1 ... + DEPTH are on their way, tile t in st[t % DEPTH]
+  for (int tile = 0; tile < ntiles; tile += DEPTH) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int t = tile + d;
+      if (d == 0 || t < ntiles) {
+        compute(t);
+        Stage& next = st[(d + 1) % DEPTH];
+        commit(next, t + 1);         // the other stage: its last readers passed the barrier before this tile
+        issue(next, t + 1 + DEPTH);
+        __syncthreads();
       }
     }
-    if (tile + 1 < ntiles) {
-      commit(tile + 1);              // the other stage: its last readers passed the barrier before this tile
-      if (tile + 2 < ntiles) issue(tile + 2);
-      load_ids(tile + 3);
-    }
-    __syncthreads();
   }
 
   // ---- merge the halves, write --------------------------------------------------------------------------------------
@@ -814,44 +866,35 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const D
     sum[c] += __shfl_xor(sum[c], 32);
     top[c] = rows.m_ref[c];
   }
-  if constexpr (WK == 2) {
-    float* other = reinterpret_cast<float*>(lds_raw) + wr * (C * 16 * (D + 4));        // [32][D + 4]: output, maximum, sum
-    if (active && wk == 1) {
+  float* other = reinterpret_cast<float*>(lds_raw) + wr * (32 * (D + 4));  // [32][D + 4]: output, maximum, sum
+  if (active && wk == 1) {
 #pragma unroll
-      for (int c = 0; c < C; ++c) {
-        float* at = other + (16 * c + col) * (D + 4);
+    for (int c = 0; c < C; ++c) {
+      float* at = other + (16 * c + col) * (D + 4);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) *(mfloat4_t*)(at + 16 * mt + 4 * kg) = rows.o[c][mt];
-        if (kg == 0) { at[D] = top[c]; at[D + 1] = sum[c]; }
-      }
-    }
-    __syncthreads();
-    if (active && wk == 0) {
-#pragma unroll
-      for (int c = 0; c < C; ++c) {
-        const float* at = other + (16 * c + col) * (D + 4);
-        const float t1 = at[D], mx = fmaxf(top[c], t1);
-        const float f0 = top[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[c] - mx);
-        const float f1 = t1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t1 - mx);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) rows.o[c][mt] = rows.o[c][mt] * f0 + *(const mfloat4_t*)(at + 16 * mt + 4 * kg) * f1;
-        sum[c] = sum[c] * f0 + at[D + 1] * f1;
-        top[c] = mx;
-      }
+      for (int mt = 0; mt < MT; ++mt) *(mfloat4_t*)(at + 16 * mt + 4 * kg) = rows.o[c][mt];
+      if (kg == 0) { at[D] = top[c]; at[D + 1] = sum[c]; }
     }
   }
+  __syncthreads();
   if (active && wk == 0) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int r = row_w + 16 * c + col;
+      const float* at = other + (16 * c + col) * (D + 4);
+      const float t1 = at[D], mx = fmaxf(top[c], t1);
+      const float f0 = top[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(top[c] - mx);
+      const float f1 = t1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t1 - mx);
+      const float total = sum[c] * f0 + at[D + 1] * f1;
       if (r >= w.live) continue;
-      const float inv = top[c] == -INFINITY ? 0.0f : 1.0f / sum[c];          // a row that saw no key: zero
+      const float inv = mx == -INFINITY ? 0.0f : 1.0f / total;               // a row that saw no key: zero
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const float x[4] = {rows.o[c][mt][0] * inv, rows.o[c][mt][1] * inv, rows.o[c][mt][2] * inv, rows.o[c][mt][3] * inv};
+        const mfloat4_t v = (rows.o[c][mt] * f0 + *(const mfloat4_t*)(at + 16 * mt + 4 * kg) * f1) * inv;
+        const float x[4] = {v[0], v[1], v[2], v[3]};
         draft_store4(p, w, r, 16 * mt + 4 * kg, D, x);
       }
-      if (p.max_partitions > 1 && kg == 0) draft_store_stats(p, w, r, top[c], sum[c]);
+      if (p.max_partitions > 1 && kg == 0) draft_store_stats(p, w, r, mx, total);
     }
   }
   if (__builtin_expect(*any_wild, 0)) draft_wild<KV, CT, D, NT>(p, w);
@@ -860,7 +903,7 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_wide_kernel(const D
 using DraftKernel = void (*)(DraftParams);
 
 // `attr_set`: one flag per device, the kernel's own (the LDS limit belongs to the kernel on one device)
-inline int launch_draft_kernel(DraftKernel kern, int lds, std::atomic<bool>* attr_set, const DraftParams& p, unsigned grid, hipStream_t st) {
+inline int launch_draft_kernel(DraftKernel kern, int threads, int lds, std::atomic<bool>* attr_set, const DraftParams& p, unsigned grid, hipStream_t st) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return fail(PA_ERR_LAUNCH, "pa_draft_attention: cannot tell the current device");
   if (!attr_set[dev].load(std::memory_order_acquire)) {
@@ -868,24 +911,29 @@ inline int launch_draft_kernel(DraftKernel kern, int lds, std::atomic<bool>* att
       return fail(PA_ERR_LAUNCH, "pa_draft_attention: cannot raise the dynamic LDS limit");
     attr_set[dev].store(true, std::memory_order_release);
   }
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(kDraftWaves * 64), lds, st, p);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(threads), lds, st, p);
   return PA_OK;
 }
 
-template <int KV, int CT, int D, int ROWS>
-int launch_draft_rows(const DraftParams& p, unsigned grid, hipStream_t st) {
+template <int KV, int CT, int D, int C>
+int launch_draft_narrow(const DraftParams& p, unsigned grid, hipStream_t st) {
   static std::atomic<bool> attr_set[64];
-  if constexpr (ROWS == 16) return launch_draft_kernel(draft_narrow_kernel<KV, CT, D>, draft_narrow_lds_bytes(D), attr_set, p, grid, st);
-  else return launch_draft_kernel(draft_wide_kernel<KV, CT, D, ROWS / 32>, draft_wide_lds_bytes(D), attr_set, p, grid, st);
+  return launch_draft_kernel(draft_narrow_kernel<KV, CT, D, C>, kDraftWaves * 64, draft_narrow_lds_bytes(D, C), attr_set, p, grid, st);
+}
+
+template <int KV, int CT, int D, int WR>
+int launch_draft_wide(const DraftParams& p, unsigned grid, hipStream_t st) {
+  static std::atomic<bool> attr_set[64];
+  return launch_draft_kernel(draft_wide_kernel<KV, CT, D, WR>, draft_wide_waves(WR) * 64, draft_wide_lds_bytes(D, WR), attr_set, p, grid, st);
 }
 
 template <int KV, int CT, int D>
 int launch_draft_dim(const DraftParams& p, int rows, unsigned grid, hipStream_t st) {
   switch (rows) {
-    case 16: return launch_draft_rows<KV, CT, D, 16>(p, grid, st);
-    case 32: return launch_draft_rows<KV, CT, D, 32>(p, grid, st);
-    case 64: return launch_draft_rows<KV, CT, D, 64>(p, grid, st);
-    default: return launch_draft_rows<KV, CT, D, 128>(p, grid, st);
+    case 16: return launch_draft_narrow<KV, CT, D, 1>(p, grid, st);
+    case 32: return launch_draft_narrow<KV, CT, D, 2>(p, grid, st);
+    case 64: return launch_draft_wide<KV, CT, D, 2>(p, grid, st);
+    default: return launch_draft_wide<KV, CT, D, 4>(p, grid, st);
   }
 }
 

@@ -22,7 +22,7 @@ import functools
 import torch
 
 from . import _native
-from .attention import (_check_cache, _code, _compute_units, _debug_tables, _int32, _known_lengths, _require_gpu, _stream_ptr,
+from .attention import (_check_cache, _code, _compute_units, _debug_tables, _int32, _require_gpu, _stream_ptr,
                         check_block_tables, reserve_decode_workspace)
 
 MAX_DRAFT_NODES = 256
@@ -108,21 +108,52 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
 
 
 # ---- how an attention launch is shaped -----------------------------------------------------------------------
-_MIN_PARTITION = 128               # tokens: one 32-token tile for each of a workgroup's 4 waves
-_MAX_PARTITIONS = 64
+# Rows (node, query head of a group) a workgroup serves from one pass over K and V -> workgroups a CU holds at once, what
+# a launch of them costs at least and what one needs per token (ns).  A launch lasts as long as its rounds of workgroups,
+# plus what the memory system needs for all of them together (bytes from HBM once, from the L2 once per row tile; what fits
+# the L2 is all but free there); a split adds the merge pass and the partial results it writes and reads.  Fitted to a sweep
+# of tiles and splits on an MI355X (batch 1 to 64, 5 to 64 nodes, 512 to 32k tokens, ratios of 2 and 8): within 10 % of the
+# best split of the sweep, 20 % at worst (launches of 20 us).
+_DRAFT_TILES = {16: (2, 5000.0, 8.5), 32: (2, 6000.0, 10.0), 64: (2, 8000.0, 17.0), 128: (1, 9000.0, 19.0)}
+_DRAFT_MERGE_NS = (4500.0, 30.0)     # the pass, per partition
+_DRAFT_HBM_BYTES_PER_NS = 6300.0
+_DRAFT_L2_BYTES_PER_NS = 14000.0
+_DRAFT_L2_HOLDS = 64 << 20
+_DRAFT_PARTIAL_BYTES_PER_NS = 4000.0
+_DRAFT_MIN_PARTITION = 128           # tokens: one 32-token tile for each of a workgroup's 4 waves
+_DRAFT_MAX_PARTITIONS = 64
 
 
 @functools.lru_cache(maxsize=4096)
-def _choose_draft_partition(batch, rows, num_kv_heads, max_keys, compute_units):
-    """(partition_size, max_partitions): the tokens of a row are cut until about two workgroups per CU exist."""
-    tiles = -(-rows // (16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128))
-    units = max(1, batch * num_kv_heads * tiles)
-    parts = min(-(-2 * compute_units // units), _MAX_PARTITIONS, -(-max_keys // _MIN_PARTITION))
-    if parts <= 1:
-        return 0, 1
-    size = -(-(-(-max_keys // parts)) // 128) * 128
-    parts = -(-max_keys // size)
-    return (size, parts) if parts > 1 else (0, 1)
+def _choose_draft_launch(batch, nodes, num_q_heads, num_kv_heads, head_dim, elem_bytes, max_keys, mean_keys, compute_units):
+    """(rows per workgroup, partition_size, max_partitions) with the smallest modelled time; (.., 0, 1): one pass."""
+    rows = nodes * (num_q_heads // num_kv_heads)
+    read = batch * num_kv_heads * mean_keys * 2.0 * head_dim * elem_bytes
+    # a batch of unequal rows: a row of the mean length counts its whole partitions and half a one at its end
+    ragged = mean_keys < 0.9 * max_keys
+    best = None
+    for tile, (per_cu, fixed, token_ns) in _DRAFT_TILES.items():
+        row_tiles = -(-rows // tile)
+        if tile > 16 and 2 * rows <= tile:
+            continue
+        memory = read / _DRAFT_HBM_BYTES_PER_NS
+        if read > _DRAFT_L2_HOLDS:
+            memory = max(memory, read * row_tiles / _DRAFT_L2_BYTES_PER_NS)
+        for want in range(1, min(_DRAFT_MAX_PARTITIONS, -(-max_keys // _DRAFT_MIN_PARTITION)) + 1):
+            size = -(-(-(-max_keys // want)) // 32) * 32
+            parts = -(-max_keys // size)
+            live = batch * (mean_keys / size + 0.5) if ragged else batch * parts
+            rounds = -(-live * num_kv_heads * row_tiles // (per_cu * compute_units))
+            compute = rounds * min(size, max_keys) * token_ns
+            # the 128-row workgroups keep two tiles of loads in flight while they multiply, the others one
+            cost = fixed + (max(memory, compute) + 0.15 * min(memory, compute) if tile == 128 else memory + compute)
+            if parts > 1:
+                partials = live * nodes * num_q_heads * head_dim * 4.0
+                cost += _DRAFT_MERGE_NS[0] + _DRAFT_MERGE_NS[1] * parts + 2.0 * partials / _DRAFT_PARTIAL_BYTES_PER_NS
+            if best is None or cost < best[0]:
+                best = (cost, tile, size, parts)
+    _, tile, size, parts = best
+    return (tile, size, parts) if parts > 1 else (tile, 0, 1)
 
 
 def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_mask, scale, k_scale=None, v_scale=None,
@@ -182,11 +213,15 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
             raise RuntimeError("%s: %d block-table entries outside the pool of %d blocks, %d rows whose tokens need more "
                                "than the table's %d columns" % (what, bad, num_blocks, short, tables.shape[1]))
     if partition_size is None:
-        bound, _ = _known_lengths(tables.shape[1] * block_size, longest_context + nodes if longest_context else None, None)
-        psize, parts = _choose_draft_partition(batch, nodes * (num_q_heads // max(1, num_kv_heads)), num_kv_heads, bound,
-                                               _compute_units(q.device))
+        bound = tables.shape[1] * block_size
+        if longest_context:
+            bound = min(bound, -(-(int(longest_context) + nodes) // 256) * 256)
+        # sixteenths of the bound: batches of about the same shape share the decision
+        mean = bound if not mean_context else max(1, min(16, round(16.0 * (mean_context + nodes) / bound))) * bound // 16
+        tile, psize, parts = _choose_draft_launch(batch, nodes, num_q_heads, max(1, num_kv_heads), head_dim, k_cache.element_size(),
+                                                  bound, mean, _compute_units(q.device))
     else:
-        psize = int(partition_size)
+        tile, psize = 0, int(partition_size)
         parts = max(1, -(-tables.shape[1] * block_size // psize)) if psize > 0 else 1
     ws_ptr, ws_bytes = None, 0
     if parts > 1:
@@ -204,7 +239,7 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
                                 tables.shape[1], lens.data_ptr(), real.data_ptr() if real is not None else None,
                                 mask.data_ptr(), mask.shape[1] * mask.shape[2] if mask.shape[0] > 1 else 0, out.data_ptr(),
                                 num_q_heads * head_dim, batch, nodes, num_q_heads, num_kv_heads, head_dim, block_size,
-                                num_blocks, float(scale), psize, parts, ws_ptr, ws_bytes, 0, _stream_ptr(q.device))
+                                num_blocks, float(scale), psize, parts, ws_ptr, ws_bytes, tile, _stream_ptr(q.device))
     _native.check(rc, "pa_draft_attention")
     return out
 

@@ -559,10 +559,11 @@ int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int6
  * A node that sees nothing (no context and an empty mask), nodes past num_nodes and rows of negative context
  * get zeros.  What a node does not see never reaches its output, NaN and infinities included.
  *   q, out               [batch, nodes, num_q_heads, head_dim] f16 / bf16 / f32, node stride in elements (rows of
- *                        the batch nodes x stride apart), 16-byte aligned rows
+ *                        the batch nodes x stride apart), 16-byte aligned rows (out: 8 bytes do for f16 / bf16)
  *   tree_mask            as pa_draft_layout writes it, rows mask_stride words apart, 0: one tree for every row
  *   max_partitions       1: one pass; > 1: the tokens of a row (committed and drafted) are cut every
- *                        partition_size tokens as in pa_decode, and a second launch merges
+ *                        partition_size tokens (a multiple of 32) as in pa_decode, at most 1024 of them, and a
+ *                        second launch merges
  *   workspace            >= pa_draft_workspace_bytes(...) bytes, 256-byte aligned, when max_partitions > 1
  *   rows_per_workgroup   (node, query head) rows of one KV head that a workgroup serves from one pass over K and
  *                        V: 16, 32, 64, 128, or 0 = the launch's own choice; never changes what is computed
