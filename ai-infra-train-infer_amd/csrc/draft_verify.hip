@@ -20,8 +20,8 @@
 //
 // Launches: (1) row statistics (z, max, the smallest kept logit; greedy: the first maximum) of every node a row
 // drafts, one workgroup a node; (2) the walk, by every workgroup of (row, slice of the vocabulary) for itself -
-// a few hundred LDS reads - and, sampling, the slice's part of the sums the draw needs, per chunk of 2048
-// entries; (3) the draw: the chunk by a scan of the sums, the token inside it.  Greedy stops after (2).
+// a few hundred LDS reads - and, sampling, the slice's part of the sums the draw needs, per chunk of 512
+// entries; (3) the draw, a wave a row: the chunk by a scan of the sums, the token inside it.  Greedy stops after (2).
 //
 // (1) for 16-bit logits is a histogram, not a pass of exponentials: a row holds at most 65536 different values, a
 // few thousand in practice, so the row's entries are counted by bit pattern in LDS (two 16-bit counters to a
@@ -43,7 +43,7 @@ constexpr int kStatThreads = 1024;
 constexpr int kStatWaves = kStatThreads / 64;
 constexpr int kWalkThreads = 256;
 constexpr int kWalkWaves = kWalkThreads / 64;
-constexpr int kChunk = 2048;                    // vocabulary entries behind one pair of stored sums
+constexpr int kChunk = 512;                     // vocabulary entries behind one pair of stored sums: a wave's, 8 a lane
 constexpr int kNodeWords = PA_MAX_DRAFT_NODES / 64;
 constexpr int kBins = 2048;                     // bins of one pass of the search
 constexpr int kVerifyMaxDevices = 64;
@@ -61,7 +61,7 @@ struct VerifyParams {
   int q_dtype;
   double c;                                     // log2(e) / T
   double top_p;
-  int nodes, vocab, chunks, chunks_per_wg;
+  int nodes, vocab, chunks, slices;             // slices: workgroups of the second launch per row
   // workspace
   double* z;                                    // [batch][nodes]
   float* top;                                   // [batch][nodes]
@@ -77,27 +77,60 @@ __device__ __forceinline__ int nodes_of(const VerifyParams& p, int b) {
   return p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
 }
 
+// 2^x for x <= 0 to 2^-51: x = n + f with |f| <= 1/2, the series of e^(f ln 2) to the 12th power (its rest is below
+// (ln 2 / 2)^13 / 13! = 2^-52.2) and the exponent added.  Below 2^-1000: 0.  Half the instructions of the library's exp2, which
+// also takes every other argument; the row statistics and the sums of the draw are bound by them.
+__device__ __forceinline__ double exp2_down(double x) {
+  const double n = __builtin_rint(x), f = x - n;
+  double r = 2.5678435993488196e-11;        // (ln 2)^12 / 12!, then (ln 2)^k / k! from k = 11 down
+  r = fma(r, f, 4.44553827187081e-10);
+  r = fma(r, f, 7.054911620801121e-09);
+  r = fma(r, f, 1.0178086009239696e-07);
+  r = fma(r, f, 1.3215486790144305e-06);
+  r = fma(r, f, 1.5252733804059838e-05);
+  r = fma(r, f, 0.00015403530393381606);
+  r = fma(r, f, 0.0013333558146428441);
+  r = fma(r, f, 0.009618129107628477);
+  r = fma(r, f, 0.055504108664821576);
+  r = fma(r, f, 0.2402265069591007);
+  r = fma(r, f, 0.6931471805599453);
+  r = fma(r, f, 1.0);
+  return x > -1000.0 ? __builtin_amdgcn_ldexp(r, (int)n) : 0.0;
+}
+
 // w of one logit; NaN and -inf weigh nothing
 __device__ __forceinline__ double logit_weight(float l, float top, double c) {
   if (l == top) return l == -INFINITY ? 0.0 : 1.0;
-  return l < top ? exp2(((double)l - (double)top) * c) : 0.0;
+  return l < top ? exp2_down(((double)l - (double)top) * c) : 0.0;
 }
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Inclusive prefix sum over the lanes of a wave, all of them active: within the rows of 16, then across them.
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp_or_zero<0x111, 0xf>(v);          // row_shr 1, 2, 4, 8: the value that many lanes down, 0 at the row's start
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);          // row_bcast 15 into rows 1 and 3
+  v += dpp_or_zero<0x143, 0xc>(v);          // row_bcast 31 into rows 2 and 3
   return v;
 }
 
-// inclusive prefix sum over the lanes of a wave
-__device__ __forceinline__ double wave_scan(double v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(v, o);
-    if (lane >= o) v += up;
-  }
-  return v;
+// One lane's value in every lane.
+__device__ __forceinline__ double wave_at(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+
+__device__ __forceinline__ double wave_sum(double v) { return wave_at(wave_scan(v), 63); }
 
 // Sum over a workgroup of WAVES waves, the same in every thread; red holds WAVES doubles.
 template <int WAVES>
@@ -116,7 +149,7 @@ __device__ __forceinline__ double group_sum(double v, double* red) {
 template <int WAVES>
 __device__ __forceinline__ double group_scan(double v, double* red) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  v = wave_scan(v, lane);
+  v = wave_scan(v);
   __syncthreads();
   if (lane == 63) red[wave] = v;
   __syncthreads();
@@ -125,7 +158,7 @@ __device__ __forceinline__ double group_scan(double v, double* red) {
 }
 
 struct StatLds {
-  double seg[1024];            // mass of 64 neighbouring values, in descending order of the values
+  double seg[1024];            // masses of neighbouring values, in descending order of the values
   double red[kStatWaves];
   double found[2];             // the crossing: mass above it, kept mass
   uint32_t key[2];             // its place
@@ -216,7 +249,9 @@ __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t*
   return r;
 }
 
-// One workgroup per node.  16-bit logits: LDS holds 32768 words of two counters, then StatLds.
+// One workgroup per node.  16-bit logits: LDS holds 32768 words, the entries of bit pattern m in the low half of word m, those
+// of -m (the same with the sign bit) counted in the high half and in the low half too; then StatLds.  32-bit logits: the bins of
+// the search, then StatLds.
 template <int DT>
 __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
@@ -225,6 +260,7 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
   if (node >= nodes_of(p, b)) return;
   constexpr bool COUNTS = DT != PA_DTYPE_F32;
   constexpr int WORDS = 32768;
+  constexpr int INF = DT == PA_DTYPE_F16 ? 0x7c00 : 0x7f80;
   uint32_t* hist = (uint32_t*)lds_raw;
   StatLds& s = *(StatLds*)(lds_raw + (COUNTS ? WORDS * 4 : kBins * 8));
   const void* ptr = (const uint8_t*)p.logits + (b * p.batch_stride + node * p.row_stride) * (COUNTS ? 2 : 4);
@@ -232,23 +268,40 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
   RowStats r;
   bool counted = false;
   if constexpr (COUNTS) {
-    constexpr uint32_t INF = DT == PA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
-    for (int i = tid; i < WORDS / 4; i += kStatThreads) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+    // The count is bound by the vector ALU: eight instructions for the addresses and increments of a pair of entries.
+    auto add = [&](uint32_t byte, uint32_t inc) __attribute__((always_inline)) {
+      __hip_atomic_fetch_add((uint32_t*)__builtin_assume_aligned(lds_raw + byte, 4), inc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    for_each_logit_pair<DT, kStatThreads, 8>(
+        ptr, p.vocab,
+        [&](uint32_t w) __attribute__((always_inline)) {
+          add((w << 2) & 0x1fffcu, ((w & 0x8000u) << 1) | 1u);
+          add((w >> 14) & 0x1fffcu, ((w >> 15) & 0x10000u) | 1u);
+        },
+        [&](uint32_t h) __attribute__((always_inline)) { add((h << 2) & 0x1fffcu, ((h & 0x8000u) << 1) | 1u); },
+        [&]() __attribute__((always_inline)) {       // while the first pieces are on their way
+          for (int i = tid; i < WORDS / 4; i += kStatThreads) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
+          __syncthreads();
+        });
     __syncthreads();
-    for_each_logit_bits<DT, kStatThreads>(ptr, p.vocab, [&](int, uint32_t bits) __attribute__((always_inline)) {
-      __hip_atomic_fetch_add(&hist[bits & 0x7fffu], (bits & 0x8000u) ? 0x10000u : 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    });
-    __syncthreads();
-    // the largest value (NaN left out), and the number of entries counted
-    uint32_t pos = 0, neg = 0xffffffffu, count = 0;       // largest m with +m (plus 1), smallest m with -m
+    // entries of +m and of -m that weigh anything
+    auto weighing = [&](int m, uint32_t& plus, uint32_t& minus) __attribute__((always_inline)) {
+      const uint32_t v = hist[m];
+      minus = v >> 16;
+      plus = (v & 0xffffu) - minus;
+      if (m == 0) { plus += minus; minus = 0; }            // -0 and +0 are one value
+      if (m >= INF) minus = 0;                             // -inf
+      if (m > INF) plus = 0;                               // NaN
+    };
+    // the largest value, and the number of entries counted
+    uint32_t pos = 0, neg = 0xffffffffu, count = 0;        // largest m with +m (plus 1), smallest m with -m
 #pragma unroll 4
     for (int i = tid; i < WORDS; i += kStatThreads) {
-      const uint32_t v = hist[i];
-      count += (v & 0xffffu) + (v >> 16);
-      if ((uint32_t)i <= INF) {
-        if ((v & 0xffffu) || (i == 0 && v)) pos = i + 1;
-        if ((v >> 16) && neg == 0xffffffffu) neg = i;
-      }
+      count += hist[i] & 0xffffu;
+      uint32_t plus, minus;
+      weighing(i, plus, minus);
+      if (plus) pos = i + 1;
+      if (minus && neg == 0xffffffffu) neg = i;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -257,6 +310,7 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       count += __shfl_xor(count, o);
     }
     if (lane == 0) { s.redu[0][wave] = pos; s.redu[1][wave] = neg; s.redu[2][wave] = count; }
+    s.seg[tid] = 0.0;
     __syncthreads();
     pos = 0; neg = 0xffffffffu; count = 0;
 #pragma unroll
@@ -265,31 +319,51 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       neg = min(neg, s.redu[1][w]);
       count += s.redu[2][w];
     }
-    counted = count == (uint32_t)p.vocab;
+    counted = count == (uint32_t)p.vocab;                  // a counter that wrapped shows in the total
     if (counted) {
-      r.top = pos ? logit_value<DT>(pos - 1) : neg < INF ? logit_value<DT>(neg | 0x8000u) : -INFINITY;
+      auto value = [](int m) { return logit_value<DT>(m); };
+      r.top = pos ? value(pos - 1) : neg != 0xffffffffu ? -value(neg) : -INFINITY;
       r.cut = -INFINITY;
-      // masses of 64 neighbouring values; segments 0..511: positive values, largest first; 512..1023: negative ones
-      auto masses = [&](int m, double& up, double& down) __attribute__((always_inline)) {
-        const uint32_t v = hist[m];
-        uint32_t a = v & 0xffffu, d = v >> 16;
-        if (m == 0) { a += d; d = 0; }                     // -0 and +0 are one value
-        if ((uint32_t)m > INF) a = d = 0;                  // NaN
-        up = a ? a * logit_weight(logit_value<DT>(m), r.top, p.c) : 0.0;
-        down = d && (uint32_t)m != INF ? d * logit_weight(logit_value<DT>(m | 0x8000u), r.top, p.c) : 0.0;
-      };
-      for (int g = wave; g < WORDS / 64; g += kStatWaves) {
-        const int m = 64 * g + lane;
+      // Groups of SPAN neighbouring m: mass of the positive values to seg[HALF - 1 - group], of the negative ones to
+      // seg[HALF + group], so that seg is in descending order of the values.  bf16: 64 (a few dozen of them hold entries, two
+      // exponentials each).  fp16, with eight times the values: 512 neighbouring ones are evenly spaced (a binade has
+      // 1024), so the weights of 64 of them are a geometric sequence - that of the largest value times the powers of
+      // exp(-spacing / T), which the group shares: three exponentials a group instead of sixteen.
+      constexpr int SPAN = DT == PA_DTYPE_F16 ? 512 : 64, HALF = WORDS / SPAN;
+      for (int g = wave; g < HALF; g += kStatWaves) {
+        uint32_t plus[SPAN / 64], minus[SPAN / 64], seen = 0;
+#pragma unroll
+        for (int k = 0; k < SPAN / 64; ++k) { weighing(SPAN * g + 64 * k + lane, plus[k], minus[k]); seen |= plus[k] | minus[k]; }
+        if (!__builtin_amdgcn_ballot_w64(seen != 0)) continue;
         double up = 0.0, down = 0.0;
-        if (__builtin_amdgcn_ballot_w64(hist[m] != 0)) {
-          masses(m, up, down);
-          up = wave_sum(up);
-          down = wave_sum(down);
+        if (SPAN == 512 && SPAN * g < INF && pos != 0 && r.top != INFINITY) {
+          const int top_m = (int)pos - 1;
+          const float gap = value(SPAN * g + 1) - value(SPAN * g);
+          const double fall_up = exp2_down(-(double)gap * p.c * (63 - lane)), fall_down = exp2_down(-(double)gap * p.c * lane);
+          // lane k < 8: the largest positive value of the k-th 64; lane 8 + k: the largest negative one
+          const int lead_m = SPAN * g + 64 * (lane & 7) + (lane < 8 ? 63 : 0);
+          const double lead = logit_weight(lane < 8 ? value(lead_m) : -value(lead_m), r.top, p.c);
+#pragma unroll
+          for (int k = 0; k < SPAN / 64; ++k) {
+            const int first = SPAN * g + 64 * k;
+            const bool own = first <= top_m && top_m < first + 63;           // the maximum leads its 64, not the last of them
+            up += plus[k] * (own ? logit_weight(value(first + lane), r.top, p.c) : wave_at(lead, k) * fall_up);
+            down += minus[k] * (wave_at(lead, 8 + k) * fall_down);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < SPAN / 64; ++k) {
+            const float x = value(SPAN * g + 64 * k + lane);
+            up += plus[k] * logit_weight(x, r.top, p.c);
+            down += minus[k] * logit_weight(-x, r.top, p.c);
+          }
         }
-        if (lane == 0) { s.seg[511 - g] = up; s.seg[512 + g] = down; }
+        up = wave_scan(up);
+        down = wave_scan(down);
+        if (lane == 63) { s.seg[HALF - 1 - g] = up; s.seg[HALF + g] = down; }
       }
       __syncthreads();
-      const double mass = s.seg[tid];
+      const double mass = s.seg[tid];                      // zero beyond 2 x HALF
       const double upto = group_scan<kStatWaves>(mass, s.red);
       if (tid == kStatThreads - 1) s.found[0] = upto;
       if (tid == 0) s.key[0] = kStatThreads;
@@ -297,25 +371,42 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       r.z = s.found[0];
       if (p.top_p < 1.0 && r.top != INFINITY && r.top != -INFINITY) {
         const double limit = p.top_p * r.z;
-        if (upto > limit) __hip_atomic_fetch_min(&s.key[0], (uint32_t)tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > limit);
+        if (past && lane == 0)
+          __hip_atomic_fetch_min(&s.key[0], (uint32_t)(64 * wave + __builtin_ctzll(past)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
-        const uint32_t o = s.key[0];                       // the first segment past the limit
-        if ((uint32_t)tid == o) s.found[0] = upto - mass;
+        const uint32_t o = s.key[0];                       // the first group past the limit
+        if ((uint32_t)tid == o) s.found[1] = upto - mass;
+        if (tid == 0) s.key[1] = SPAN;
         __syncthreads();
-        if (o < kStatThreads) {
-          // inside the segment, lanes in descending order of the values
-          const int m = o < 512 ? 64 * (511 - (int)o) + 63 - lane : 64 * ((int)o - 512) + lane;
-          double up, down;
-          masses(m, up, down);
-          const double here = o < 512 ? up : down;
-          const double to = s.found[0] + wave_scan(here, lane);
-          unsigned long long hit = __builtin_amdgcn_ballot_w64(here > 0.0 && to > limit);
-          const unsigned long long some = __builtin_amdgcn_ballot_w64(here > 0.0);
-          // the first value whose mass crosses the limit; by rounding none: the segment's last
-          const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some | 1ull);
-          r.z = __shfl(to, l);
-          const uint32_t mb = __shfl(m, l);
-          r.cut = logit_value<DT>(o < 512 ? mb : mb | 0x8000u);
+        if (o < 2 * HALF) {
+          // its values in descending order: wave k has the k-th 64 of them, then their masses and those in front
+          const bool positive = o < HALF;
+          const int first = SPAN * (positive ? HALF - 1 - (int)o : (int)o - HALF);
+          double here = 0.0;
+          int m = 0;
+          if (wave < SPAN / 64) {
+            m = positive ? first + SPAN - 1 - 64 * wave - lane : first + 64 * wave + lane;
+            uint32_t plus, minus;
+            weighing(m, plus, minus);
+            here = positive ? plus * logit_weight(value(m), r.top, p.c) : minus * logit_weight(-value(m), r.top, p.c);
+          }
+          double to = wave_scan(here);
+          if (lane == 63) s.red[wave] = to;
+          __syncthreads();
+          to += s.found[1];
+          for (int k = 0; k < wave; ++k) to += s.red[k];
+          if (here > 0.0 && to > limit)
+            __hip_atomic_fetch_min(&s.key[1], (uint32_t)(64 * wave + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          __syncthreads();
+          // the first value past the limit; where rounding leaves none the whole group stays
+          if ((uint32_t)(64 * wave + lane) == min(s.key[1], (uint32_t)SPAN - 1)) {
+            s.found[0] = to;
+            s.redu[0][0] = __float_as_uint(positive ? value(m) : -value(m));
+          }
+          __syncthreads();
+          r.z = s.found[0];
+          r.cut = __uint_as_float(s.redu[0][0]);
         }
       }
     }
@@ -360,14 +451,41 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_argmax_kernel(const Ve
 }
 
 struct WalkLds {
+  double z[PA_MAX_DRAFT_NODES];      // the nodes' row statistics
+  float top[PA_MAX_DRAFT_NODES];
+  float cut[PA_MAX_DRAFT_NODES];
   double w[PA_MAX_DRAFT_NODES];      // the node's weight in its parent's row; drafts drawn from q: its weight / q
-  double red[2][kWalkWaves];
   int parent[PA_MAX_DRAFT_NODES];
   int token[PA_MAX_DRAFT_NODES];
   float u[PA_MAX_DRAFT_NODES];
   int path[PA_MAX_DRAFT_NODES];
-  uint64_t skip[kChunk / 64];        // entries of the chunk that the draw leaves out
 };
+
+// Entries i0 ... i0 + 7 of a row as floats (beyond its end: `beyond`), in 16-byte loads where they are aligned.
+__device__ __forceinline__ void load_entries(const void* row, int dtype, int i0, int vocab, float beyond, float (&x)[8]) {
+  const int es = dtype == PA_DTYPE_F32 ? 4 : 2;
+  if (i0 >= vocab) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = beyond;
+  } else if (i0 + 8 <= vocab && ((reinterpret_cast<uintptr_t>(row) + (uintptr_t)i0 * es) & 15u) == 0) {
+    load8_as_f32(row, i0, dtype, x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = i0 + e < vocab ? load_as_f32(row, i0 + e, dtype) : beyond;
+  }
+}
+
+// The weights with which the token after node `last` is drawn, of 8 entries of logits l, and all kept weights.
+// drop: bit e leaves entry e out (a refused child's token).  from_q: drafts drawn from q were refused; inv_z: 1 / z then.
+__device__ __forceinline__ void draw_weights(const VerifyParams& p, const float (&l)[8], const float (&q)[8], bool from_q, float top,
+                                             float cut, double inv_z, uint32_t drop, double (&drawn)[8], double (&all)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    all[e] = l[e] >= cut ? logit_weight(l[e], top, p.c) : 0.0;
+    if (from_q) drawn[e] = fmax(fma(all[e], inv_z, -(double)q[e]), 0.0);
+    else drawn[e] = (drop >> e) & 1u ? 0.0 : all[e];
+  }
+}
 
 // The walk of one row.  Every wave does the same from the same LDS values, so its result is uniform; lane l
 // stands for nodes l, 64 + l, ...  Returns the last accepted node; s.path and `count` hold the way there, `refused`
@@ -380,7 +498,7 @@ __device__ __forceinline__ int walk(const VerifyParams& p, WalkLds& s, int b, in
   count = 1;
   if (threadIdx.x == 0) s.path[0] = 0;
   for (;;) {
-    const double z = GREEDY ? 0.0 : p.z[(int64_t)b * p.nodes + cur];
+    const double z = GREEDY ? 0.0 : s.z[cur];
     double left = z;
     int next = -1;
 #pragma unroll
@@ -416,8 +534,8 @@ __device__ __forceinline__ int walk(const VerifyParams& p, WalkLds& s, int b, in
   }
 }
 
-__device__ __forceinline__ float draft_prob(const VerifyParams& p, int b, int node, int64_t token) {
-  return load_as_f32(p.q, b * p.q_batch_stride + node * p.q_row_stride + token, p.q_dtype);
+__device__ __forceinline__ const void* draft_probs_row(const VerifyParams& p, int b, int node) {
+  return (const uint8_t*)p.q + (b * p.q_batch_stride + node * p.q_row_stride) * (p.q_dtype == PA_DTYPE_F32 ? 4 : 2);
 }
 
 // One workgroup per (slice of the vocabulary, row): the walk, the row's outputs (slice 0) and the slice's sums.
@@ -438,6 +556,10 @@ __global__ __launch_bounds__(kWalkThreads) void draft_walk_kernel(const VerifyPa
   const uint8_t* rows = (const uint8_t*)p.logits + b * p.batch_stride * ES;
   {
     const int i = tid;                    // kWalkThreads == PA_MAX_DRAFT_NODES
+    if (i < n) {
+      if (!GREEDY) { s.z[i] = p.z[at + i]; s.top[i] = p.top[at + i]; }
+      s.cut[i] = p.cut[at + i];
+    }
     int up = -1, tok = -1;
     double w = 0.0;
     if (i > 0 && i < n) {
@@ -453,7 +575,7 @@ __global__ __launch_bounds__(kWalkThreads) void draft_walk_kernel(const VerifyPa
           if (l >= p.cut[at + up]) w = logit_weight(l, p.top[at + up], p.c);
           if (p.q) {
             // u * q * z < w  <=>  u * z < w / q; a token that the draft cannot draw passes if it has any weight
-            const double qv = draft_prob(p, b, up, tok);
+            const double qv = load_as_f32(draft_probs_row(p, b, up), tok, p.q_dtype);
             w = qv > 0.0 ? w / qv : w > 0.0 ? (double)INFINITY : 0.0;
           }
         }
@@ -475,166 +597,170 @@ __global__ __launch_bounds__(kWalkThreads) void draft_walk_kernel(const VerifyPa
       // the drawn token's place is the third launch's (greedy: this one's)
       if (i + 1 < count) p.out_tokens[at + i] = p.tokens[at + s.path[i + 1]];
       else if (i >= count) p.out_tokens[at + i] = -1;
-      else if (GREEDY) p.out_tokens[at + i] = __float_as_int(p.cut[at + last]);
+      else if (GREEDY) p.out_tokens[at + i] = __float_as_int(s.cut[last]);
     }
     if (tid == 0) { p.out_counts[b] = count; if (!GREEDY) p.last[b] = last; }
   }
   if constexpr (!GREEDY) {
+    const int lane = tid & 63;
     bool any = false;
+    int gone[kNodeWords];                    // this lane's refused children of the last node: their tokens
 #pragma unroll
-    for (int x = 0; x < kNodeWords; ++x) any = any || refused[x] != 0;
-    const float top = p.top[at + last], cut = p.cut[at + last];
-    const double z = p.z[at + last];
-    const uint8_t* row = rows + last * p.row_stride * ES;
-    const int first = blockIdx.x * p.chunks_per_wg, end = min(first + p.chunks_per_wg, p.chunks);
-    for (int chunk = first; chunk < end; ++chunk) {
+    for (int x = 0; x < kNodeWords; ++x) {
+      any = any || refused[x] != 0;
+      gone[x] = (refused[x] >> lane) & 1ull ? s.token[64 * x + lane] : -1;
+    }
+    const float top = s.top[last], cut = s.cut[last];
+    const void* row = rows + last * p.row_stride * ES;
+    const void* q_row = any && p.q ? draft_probs_row(p, b, last) : nullptr;
+    const double inv_z = q_row ? 1.0 / s.z[last] : 0.0;
+    // a wave takes chunks of 512 entries by itself, 8 consecutive ones a lane, the next chunk's on their way
+    const int waves = gridDim.x * kWalkWaves;
+    float l[8], q[8] = {};
+    auto load = [&](int chunk) __attribute__((always_inline)) {
+      const int i0 = chunk < p.chunks ? chunk * kChunk + lane * 8 : p.vocab;
+      load_entries(row, DT, i0, p.vocab, -INFINITY, l);
+      if (q_row) load_entries(q_row, p.q_dtype, i0, p.vocab, 0.0f, q);
+    };
+    int chunk = blockIdx.x * kWalkWaves + (tid >> 6);
+    load(chunk);
+    for (; chunk < p.chunks; chunk += waves) {
       const int base = chunk * kChunk;
-      __syncthreads();
+      uint32_t drop = 0;
       if (any && !p.q) {
-        for (int i = tid; i < kChunk / 64; i += kWalkThreads) s.skip[i] = 0;
-        __syncthreads();
-        uint64_t mine = 0;
 #pragma unroll
-        for (int x = 0; x < kNodeWords; ++x)
-          if (x == (tid >> 6)) mine = refused[x];
-        if ((mine >> (tid & 63)) & 1ull) {
-          const int off = s.token[tid] - base;
-          if (off >= 0 && off < kChunk) __hip_atomic_fetch_or(&s.skip[off >> 6], 1ull << (off & 63), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        }
-        __syncthreads();
-      }
-      double drawn = 0.0, all = 0.0;
-#pragma unroll
-      for (int k = 0; k < kChunk / kWalkThreads; ++k) {
-        const int off = k * kWalkThreads + tid, i = base + off;
-        if (i < p.vocab) {
-          const float l = load_as_f32(row, i, DT);
-          const double w = l >= cut ? logit_weight(l, top, p.c) : 0.0;
-          all += w;
-          if (any) {
-            if (p.q) drawn += fmax(w / z - (double)draft_prob(p, b, last, i), 0.0);
-            else if (!((s.skip[off >> 6] >> (off & 63)) & 1ull)) drawn += w;
+        for (int x = 0; x < kNodeWords; ++x) {
+          unsigned long long here = __builtin_amdgcn_ballot_w64(gone[x] >= base && gone[x] < base + kChunk);
+          while (here) {
+            const int off = __builtin_amdgcn_readlane(gone[x], __builtin_ctzll(here)) - base;
+            here &= here - 1;
+            if ((off >> 3) == lane) drop |= 1u << (off & 7);
           }
         }
       }
-      drawn = wave_sum(drawn);
-      all = wave_sum(all);
-      if ((tid & 63) == 0) { s.red[0][tid >> 6] = drawn; s.red[1][tid >> 6] = all; }
-      __syncthreads();
-      if (tid == 0) {
-        double d = 0.0, a = 0.0;
+      float l_now[8], q_now[8];
 #pragma unroll
-        for (int w = 0; w < kWalkWaves; ++w) { d += s.red[0][w]; a += s.red[1][w]; }
+      for (int e = 0; e < 8; ++e) { l_now[e] = l[e]; q_now[e] = q[e]; }
+      load(chunk + waves);
+      double d = 0.0, a = 0.0, drawn[8], all[8];
+      draw_weights(p, l_now, q_now, q_row != nullptr, top, cut, inv_z, drop, drawn, all);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) { d += drawn[e]; a += all[e]; }
+      d = wave_sum(d);
+      a = wave_sum(a);
+      if (lane == 0) {
         double* out = p.sums + ((int64_t)b * p.chunks + chunk) * 2;
-        out[0] = any ? d : a;
+        out[0] = d;
         out[1] = a;
       }
     }
   }
 }
 
-// One workgroup per row: the token drawn after the last accepted node.
+// One wave per row: the token drawn after the last accepted node.
 template <int DT>
-__global__ __launch_bounds__(kWalkThreads) void draft_draw_kernel(const VerifyParams p) {
-  __shared__ double red[kWalkWaves];
-  __shared__ double run;                 // weight before the chunk
-  __shared__ int where, tail;
-  __shared__ uint64_t skip[kChunk / 64];
+__global__ __launch_bounds__(64) void draft_draw_kernel(const VerifyParams p) {
   constexpr int ES = DT == PA_DTYPE_F32 ? 4 : 2;
-  constexpr int PER = kChunk / kWalkThreads;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const int last = p.last[b];
-  if (last < 0) return;
+  const int b = blockIdx.x, lane = threadIdx.x;
   const int64_t at = (int64_t)b * p.nodes;
+  const int last = p.last[b], count = p.out_counts[b];
+  if (last < 0) return;
   const int n = nodes_of(p, b);
-  const double* sums = p.sums + (int64_t)b * p.chunks * 2;
-  // what is left after the refused children, or all that is kept if nothing is
-  double mine[2] = {0.0, 0.0};
-  for (int i = tid; i < p.chunks; i += kWalkThreads) { mine[0] += sums[2 * i]; mine[1] += sums[2 * i + 1]; }
-  const double left = group_sum<kWalkWaves>(mine[0], red);
-  const double kept = group_sum<kWalkWaves>(mine[1], red);
-  const int side = left > 0.0 ? 0 : 1;
-  const double target = (double)p.uniforms[at] * (side == 0 ? left : kept);
-  // the first chunk in which the running sum passes the target; the last that holds any weight if none does
-  if (tid == 0) { where = p.chunks; tail = 0; }
-  __syncthreads();
-  double before = 0.0;
-  for (int base = 0; base < p.chunks; base += kWalkThreads) {
-    const int i = base + tid;
-    const double v = i < p.chunks ? sums[2 * i + side] : 0.0;
-    const double upto = before + group_scan<kWalkWaves>(v, red);
-    if (v > 0.0) {
-      atomicMax(&tail, i);
-      if (upto > target) atomicMin(&where, i);
-    }
-    __syncthreads();
-    if (where < p.chunks) {
-      if (i == where) run = upto - v;
-      break;
-    }
-    double all = 0.0;
-#pragma unroll
-    for (int w = 0; w < kWalkWaves; ++w) all += red[w];
-    before += all;
-    __syncthreads();
-  }
-  __syncthreads();
-  const bool crossed = where < p.chunks;
-  const int chunk = crossed ? where : tail;
-  const int base = chunk * kChunk;
-  // children of the last node: refused every one, their tokens are left out
-  for (int i = tid; i < kChunk / 64; i += kWalkThreads) skip[i] = 0;
-  __syncthreads();
-  int up = -1;
-  if (tid > 0 && tid < n) {
-    up = p.parents ? p.parents[b * p.parents_stride + tid] : tid - 1;
-    if (up >= tid) up = -1;
-  }
-  const bool any = __syncthreads_or(up == last);
-  if (up == last && !p.q) {
-    const int64_t off = p.tokens[at + tid] - base;
-    if (off >= 0 && off < kChunk) __hip_atomic_fetch_or(&skip[off >> 6], 1ull << (off & 63), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-  }
-  __syncthreads();
   const float top = p.top[at + last], cut = p.cut[at + last];
-  const double z = p.z[at + last];
-  const uint8_t* row = (const uint8_t*)p.logits + (b * p.batch_stride + last * p.row_stride) * ES;
-  // index order: thread t holds entries PER t ... of the chunk
-  double w[PER], sum = 0.0;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    const int off = tid * PER + k, i = base + off;
-    w[k] = 0.0;
-    if (i < p.vocab) {
-      const float l = load_as_f32(row, i, DT);
-      w[k] = l >= cut ? logit_weight(l, top, p.c) : 0.0;
-      if (side == 0 && any) {
-        if (p.q) w[k] = fmax(w[k] / z - (double)draft_prob(p, b, last, i), 0.0);
-        else if ((skip[off >> 6] >> (off & 63)) & 1ull) w[k] = 0.0;
+  const double z = p.z[at + last], u = (double)p.uniforms[at];
+  const double2* sums = (const double2*)(p.sums + (int64_t)b * p.chunks * 2);
+  // what is left after the refused children, or all that is kept if nothing is: lane l adds up chunks l * per ...
+  const int per = (p.chunks + 63) / 64;
+  double left = 0.0, kept = 0.0;
+  for (int i = lane * per; i < min((lane + 1) * per, p.chunks); ++i) {
+    const double2 v = sums[i];
+    left += v.x;
+    kept += v.y;
+  }
+  const double left_to = wave_scan(left), kept_to = wave_scan(kept);
+  const double left_all = wave_at(left_to, 63);
+  const bool rest = left_all > 0.0;
+  const double target = u * (rest ? left_all : wave_at(kept_to, 63));
+  const double mine = rest ? left : kept, to = rest ? left_to : kept_to;
+  // the first chunk in which the running sum passes the target; by rounding none: the last that holds any weight
+  const unsigned long long some = __builtin_amdgcn_ballot_w64(mine > 0.0);
+  unsigned long long hit = __builtin_amdgcn_ballot_w64(mine > 0.0 && to > target);
+  if (!some) {                               // nothing at all (a row without a finite logit): the first token
+    if (lane == 0) p.out_tokens[at + count - 1] = 0;
+    return;
+  }
+  const int owner = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(some);
+  double run = wave_at(to, owner) - wave_at(mine, owner);      // weight before the chunk
+  int chunk = -1, tail = owner * per;
+  double before = run;
+  for (int i0 = owner * per; i0 < min((owner + 1) * per, p.chunks) && chunk < 0; i0 += 64) {
+    const int i = i0 + lane;
+    double m = 0.0;
+    if (i < min((owner + 1) * per, p.chunks)) m = rest ? sums[i].x : sums[i].y;
+    const double upto = before + wave_scan(m);
+    const unsigned long long weight = __builtin_amdgcn_ballot_w64(m > 0.0);
+    const unsigned long long past = __builtin_amdgcn_ballot_w64(m > 0.0 && upto > target);
+    if (past || weight) {
+      const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(weight);
+      run = wave_at(upto, l) - wave_at(m, l);
+      tail = i0 + l;
+      if (past) chunk = tail;
+    }
+    before = wave_at(upto, 63);
+  }
+  if (chunk < 0) chunk = tail;
+  // inside the chunk: lane l holds entries 8 l ... of it
+  const int base = chunk * kChunk;
+  uint32_t drop = 0;
+  bool any = false;
+  for (int c0 = 0; c0 < n; c0 += 64) {
+    const int c = c0 + lane;
+    int gone = -1;
+    if (c > 0 && c < n) {
+      const int up = p.parents ? p.parents[b * p.parents_stride + c] : c - 1;
+      if (up == last) {                      // < c: `last` is one of the row's nodes, and a parent past the node is none
+        any = any || last < c;
+        const int64_t t = p.tokens[at + c];
+        if (last < c && t >= base && t < base + kChunk) gone = (int)t - base;
       }
     }
-    sum += w[k];
-  }
-  if (tid == 0) { where = kChunk; tail = -1; }
-  double upto = (crossed ? run : 0.0) + group_scan<kWalkWaves>(sum, red) - sum;
-  int hit = kChunk, some = -1;
-#pragma unroll
-  for (int k = 0; k < PER; ++k) {
-    upto += w[k];
-    if (w[k] > 0.0) {
-      some = tid * PER + k;
-      if (crossed && upto > target && hit == kChunk) hit = tid * PER + k;
+    unsigned long long here = __builtin_amdgcn_ballot_w64(gone >= 0);
+    while (here) {
+      const int off = __builtin_amdgcn_readlane(gone, __builtin_ctzll(here));
+      here &= here - 1;
+      if ((off >> 3) == lane) drop |= 1u << (off & 7);
     }
   }
-  __syncthreads();
-  if (hit < kChunk) atomicMin(&where, hit);
-  if (some >= 0) atomicMax(&tail, some);
-  __syncthreads();
-  if (tid == 0) {
-    // rounding left the target at or above the chunk's sum: its last entry with any weight
-    const int off = where < kChunk ? where : max(tail, 0);
-    p.out_tokens[at + p.out_counts[b] - 1] = min(base + off, p.vocab - 1);
+  any = __builtin_amdgcn_ballot_w64(any) != 0;
+  const void* row = (const uint8_t*)p.logits + (b * p.batch_stride + last * p.row_stride) * ES;
+  const void* q_row = any && p.q ? draft_probs_row(p, b, last) : nullptr;
+  double drawn[8], all[8], sum = 0.0;
+  const int i0 = base + lane * 8;
+  float l[8], q[8] = {};
+  load_entries(row, DT, i0, p.vocab, -INFINITY, l);
+  if (q_row) load_entries(q_row, p.q_dtype, i0, p.vocab, 0.0f, q);
+  draw_weights(p, l, q, q_row != nullptr, top, cut, q_row ? 1.0 / z : 0.0, drop, drawn, all);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    drawn[e] = rest ? drawn[e] : all[e];
+    sum += drawn[e];
   }
+  double upto = run + (wave_scan(sum) - sum);
+  int first = 8, final = -1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    upto += drawn[e];
+    if (drawn[e] > 0.0) {
+      final = e;
+      if (upto > target && first == 8) first = e;
+    }
+  }
+  hit = __builtin_amdgcn_ballot_w64(first < 8);
+  const unsigned long long any_weight = __builtin_amdgcn_ballot_w64(final >= 0);
+  // rounding left the target at or above the chunk's sum: its last entry with any weight
+  const int from = hit ? __builtin_ctzll(hit) : any_weight ? 63 - __builtin_clzll(any_weight) : 0;
+  const int off = from * 8 + max(__builtin_amdgcn_readlane(hit ? first : final, from), 0);
+  if (lane == 0) p.out_tokens[at + count - 1] = min(base + off, p.vocab - 1);
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -677,9 +803,8 @@ static int launch_verify(const VerifyParams& p, int64_t batch, bool greedy, hipS
     attr_set[dev].store(true, std::memory_order_release);
   }
   hipLaunchKernelGGL(kern, rows, dim3(kStatThreads), lds, st, p);
-  const unsigned slices = (unsigned)((p.chunks + p.chunks_per_wg - 1) / p.chunks_per_wg);
-  hipLaunchKernelGGL((draft_walk_kernel<DT, false>), dim3(slices, (unsigned)batch), dim3(kWalkThreads), 0, st, p);
-  hipLaunchKernelGGL(draft_draw_kernel<DT>, dim3((unsigned)batch), dim3(kWalkThreads), 0, st, p);
+  hipLaunchKernelGGL((draft_walk_kernel<DT, false>), dim3((unsigned)p.slices, (unsigned)batch), dim3(kWalkThreads), 0, st, p);
+  hipLaunchKernelGGL(draft_draw_kernel<DT>, dim3((unsigned)batch), dim3(64), 0, st, p);
   return check_launch("pa_verify_drafts");
 }
 
@@ -744,9 +869,10 @@ extern "C" int pa_verify_drafts(const void* logits, int dtype, int64_t row_strid
   p.nodes = (int)nodes;
   p.vocab = (int)vocab;
   p.chunks = (int)((vocab + kChunk - 1) / kChunk);
-  // about 512 workgroups of the second launch, at least one chunk each
-  const int64_t want = (512 + batch - 1) / batch;
-  p.chunks_per_wg = (int)((p.chunks + want - 1) / want);
+  // as many workgroups of the second launch as the GPU holds at once (six per CU): a wave's chunks are a chain of loads and
+  // sums, so fewer of them each (512 workgroups: 32 us for 64 rows of 152k entries with draft probabilities)
+  const int64_t want = (1536 + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
+  p.slices = (int)(want < most ? want : most);
   p.z = (double*)(ws + l.z);
   p.top = (float*)(ws + l.top);
   p.cut = (float*)(ws + l.cut);
