@@ -82,8 +82,9 @@ SIGNATURES = {
 # null pointer and floats for floats, which is all the module accepts; every other entry, and every
 # entry when the module is missing, goes through ctypes.
 FAST_ENTRIES = ("pa_decode", "pa_decode_shared_prefix", "pa_qk_norm_rope_store", "pa_add_rms_norm", "pa_silu_mul",
-                "pa_kv_store", "pa_kv_store_fp8", "pa_prefill", "pa_sample")
-_KIND = {_ptr: "p", _i64: "q", _int: "i", _f32: "f"}
+                "pa_kv_store", "pa_kv_store_fp8", "pa_prefill", "pa_sample", "pa_draft_layout", "pa_draft_attention",
+                "pa_verify_drafts", "pa_draft_commit")
+_KIND = {_ptr: "p", _i64: "q", _int: "i", _f32: "f", _f64: "d"}
 
 
 class _Library:

@@ -81,27 +81,42 @@ __device__ __forceinline__ int nodes_of(const VerifyParams& p, int b) {
 // (ln 2 / 2)^13 / 13! = 2^-52.2) and the exponent added.  Below 2^-1000: 0.  Half the instructions of the library's exp2, which
 // also takes every other argument; the row statistics and the sums of the draw are bound by them.
 __device__ __forceinline__ double exp2_down(double x) {
+  // (ln 2)^k / k!, held in scalar registers: as literals each costs two moves into the accumulator of its multiply-add
+  double c12 = 2.5678435993488196e-11;
+  double c11 = 4.44553827187081e-10;
+  double c10 = 7.054911620801121e-09;
+  double c9 = 1.0178086009239696e-07;
+  double c8 = 1.3215486790144305e-06;
+  double c7 = 1.5252733804059838e-05;
+  double c6 = 0.00015403530393381606;
+  double c5 = 0.0013333558146428441;
+  double c4 = 0.009618129107628477;
+  double c3 = 0.055504108664821576;
+  double c2 = 0.2402265069591007;
+  double c1 = 0.6931471805599453;
+  asm("" : "+s"(c12), "+s"(c11), "+s"(c10), "+s"(c9), "+s"(c8), "+s"(c7));
+  asm("" : "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3), "+s"(c2), "+s"(c1));
   const double n = __builtin_rint(x), f = x - n;
-  double r = 2.5678435993488196e-11;        // (ln 2)^12 / 12!, then (ln 2)^k / k! from k = 11 down
-  r = fma(r, f, 4.44553827187081e-10);
-  r = fma(r, f, 7.054911620801121e-09);
-  r = fma(r, f, 1.0178086009239696e-07);
-  r = fma(r, f, 1.3215486790144305e-06);
-  r = fma(r, f, 1.5252733804059838e-05);
-  r = fma(r, f, 0.00015403530393381606);
-  r = fma(r, f, 0.0013333558146428441);
-  r = fma(r, f, 0.009618129107628477);
-  r = fma(r, f, 0.055504108664821576);
-  r = fma(r, f, 0.2402265069591007);
-  r = fma(r, f, 0.6931471805599453);
+  double r = fma(c12, f, c11);
+  r = fma(r, f, c10);
+  r = fma(r, f, c9);
+  r = fma(r, f, c8);
+  r = fma(r, f, c7);
+  r = fma(r, f, c6);
+  r = fma(r, f, c5);
+  r = fma(r, f, c4);
+  r = fma(r, f, c3);
+  r = fma(r, f, c2);
+  r = fma(r, f, c1);
   r = fma(r, f, 1.0);
   return x > -1000.0 ? __builtin_amdgcn_ldexp(r, (int)n) : 0.0;
 }
 
 // w of one logit; NaN and -inf weigh nothing
 __device__ __forceinline__ double logit_weight(float l, float top, double c) {
-  if (l == top) return l == -INFINITY ? 0.0 : 1.0;
-  return l < top ? exp2_down(((double)l - (double)top) * c) : 0.0;
+  const double x = l == top ? 0.0 : (double)l - (double)top;
+  const double w = exp2_down(x * c);
+  return l <= top && l > -INFINITY ? w : 0.0;
 }
 
 template <int CTRL, int ROWS>
@@ -158,7 +173,7 @@ __device__ __forceinline__ double group_scan(double v, double* red) {
 }
 
 struct StatLds {
-  double seg[1024];            // masses of neighbouring values, in descending order of the values
+  double seg[128];             // masses of 512 neighbouring values, in descending order of the values
   double red[kStatWaves];
   double found[2];             // the crossing: mass above it, kept mass
   uint32_t key[2];             // its place
@@ -265,8 +280,6 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
   StatLds& s = *(StatLds*)(lds_raw + (COUNTS ? WORDS * 4 : kBins * 8));
   const void* ptr = (const uint8_t*)p.logits + (b * p.batch_stride + node * p.row_stride) * (COUNTS ? 2 : 4);
   const int64_t at = (int64_t)b * p.nodes + node;
-  RowStats r;
-  bool counted = false;
   if constexpr (COUNTS) {
     // The count is bound by the vector ALU: eight instructions for the addresses and increments of a pair of entries.
     auto add = [&](uint32_t byte, uint32_t inc) __attribute__((always_inline)) {
@@ -284,24 +297,42 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
           __syncthreads();
         });
     __syncthreads();
+    // A wave takes blocks of 512 neighbouring m (wave, 16 + wave, ...), 8 consecutive ones a lane.
+    // Most blocks are empty and cost a read and a test.
+    constexpr int BLOCKS = WORDS / 512, MINE = BLOCKS / kStatWaves;
+    bool seen[MINE];
+    auto words = [&](int m0, uint32_t (&v)[8]) __attribute__((always_inline)) {
+      const uint4 x = ((const uint4*)hist)[m0 / 4], y = ((const uint4*)hist)[m0 / 4 + 1];
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    };
     // entries of +m and of -m that weigh anything
-    auto weighing = [&](int m, uint32_t& plus, uint32_t& minus) __attribute__((always_inline)) {
-      const uint32_t v = hist[m];
-      minus = v >> 16;
-      plus = (v & 0xffffu) - minus;
+    auto weighing = [&](uint32_t word, int m, uint32_t& plus, uint32_t& minus) __attribute__((always_inline)) {
+      minus = word >> 16;
+      plus = (word & 0xffffu) - minus;
       if (m == 0) { plus += minus; minus = 0; }            // -0 and +0 are one value
       if (m >= INF) minus = 0;                             // -inf
       if (m > INF) plus = 0;                               // NaN
     };
     // the largest value, and the number of entries counted
     uint32_t pos = 0, neg = 0xffffffffu, count = 0;        // largest m with +m (plus 1), smallest m with -m
-#pragma unroll 4
-    for (int i = tid; i < WORDS; i += kStatThreads) {
-      count += hist[i] & 0xffffu;
-      uint32_t plus, minus;
-      weighing(i, plus, minus);
-      if (plus) pos = i + 1;
-      if (minus && neg == 0xffffffffu) neg = i;
+#pragma unroll
+    for (int k = 0; k < MINE; ++k) {
+      uint32_t v[8], any = 0;
+      const int m0 = (wave + kStatWaves * k) * 512 + lane * 8;
+      words(m0, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) any |= v[j];
+      seen[k] = __builtin_amdgcn_ballot_w64(any != 0) != 0;
+      if (!seen[k]) continue;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t plus, minus;
+        weighing(v[j], m0 + j, plus, minus);
+        count += v[j] & 0xffffu;
+        if (plus) pos = m0 + j + 1;
+        if (minus) neg = min(neg, (uint32_t)(m0 + j));
+      }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -310,7 +341,6 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       count += __shfl_xor(count, o);
     }
     if (lane == 0) { s.redu[0][wave] = pos; s.redu[1][wave] = neg; s.redu[2][wave] = count; }
-    s.seg[tid] = 0.0;
     __syncthreads();
     pos = 0; neg = 0xffffffffu; count = 0;
 #pragma unroll
@@ -319,102 +349,111 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       neg = min(neg, s.redu[1][w]);
       count += s.redu[2][w];
     }
-    counted = count == (uint32_t)p.vocab;                  // a counter that wrapped shows in the total
+    // a counter that wrapped shows in the total; rows whose maximum is infinite are searched too
+    const bool counted = count == (uint32_t)p.vocab && pos != INF + 1;
+    if (counted && pos == 0 && neg == 0xffffffffu) {       // nothing weighs anything
+      if (tid == 0) { p.z[at] = 0.0; p.top[at] = p.cut[at] = -INFINITY; }
+      return;
+    }
     if (counted) {
       auto value = [](int m) { return logit_value<DT>(m); };
-      r.top = pos ? value(pos - 1) : neg != 0xffffffffu ? -value(neg) : -INFINITY;
-      r.cut = -INFINITY;
-      // Groups of SPAN neighbouring m: mass of the positive values to seg[HALF - 1 - group], of the negative ones to
-      // seg[HALF + group], so that seg is in descending order of the values.  bf16: 64 (a few dozen of them hold entries, two
-      // exponentials each).  fp16, with eight times the values: 512 neighbouring ones are evenly spaced (a binade has
-      // 1024), so the weights of 64 of them are a geometric sequence - that of the largest value times the powers of
-      // exp(-spacing / T), which the group shares: three exponentials a group instead of sixteen.
-      constexpr int SPAN = DT == PA_DTYPE_F16 ? 512 : 64, HALF = WORDS / SPAN;
-      for (int g = wave; g < HALF; g += kStatWaves) {
-        uint32_t plus[SPAN / 64], minus[SPAN / 64], seen = 0;
+      const float top = pos ? value(pos - 1) : -value(neg);
+      const int top_up = (int)pos - 1, top_down = pos ? 0 : (int)neg;
+      // Masses of a lane's 8 values of one sign, largest value first.  They are evenly spaced (a binade has 128 values or
+      // more), so their weights are a geometric sequence from that of the largest one not above the maximum.
+      auto masses_up = [&](int m0, double (&mass)[8]) __attribute__((always_inline)) {
+        uint32_t w8[8];
+        words(m0, w8);
+        const double fall = exp2_down(-(double)(value(m0 + 1) - value(m0)) * p.c);
+        double w = logit_weight(value(min(m0 + 7, max(top_up, 0))), top, p.c);
 #pragma unroll
-        for (int k = 0; k < SPAN / 64; ++k) { weighing(SPAN * g + 64 * k + lane, plus[k], minus[k]); seen |= plus[k] | minus[k]; }
-        if (!__builtin_amdgcn_ballot_w64(seen != 0)) continue;
+        for (int j = 7; j >= 0; --j) {
+          uint32_t plus, minus;
+          weighing(w8[j], m0 + j, plus, minus);
+          const bool real = m0 + j <= top_up && m0 < INF;
+          mass[7 - j] = real ? plus * w : 0.0;
+          w = real ? w * fall : w;
+        }
+      };
+      auto masses_down = [&](int m0, double (&mass)[8]) __attribute__((always_inline)) {
+        uint32_t w8[8];
+        words(m0, w8);
+        const double fall = exp2_down(-(double)(value(m0 + 1) - value(m0)) * p.c);
+        double w = logit_weight(-value(max(m0, top_down)), top, p.c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t plus, minus;
+          weighing(w8[j], m0 + j, plus, minus);
+          const bool real = m0 + j >= top_down && m0 < INF;
+          mass[j] = real ? minus * w : 0.0;
+          w = real ? w * fall : w;
+        }
+      };
+      auto sum8 = [](const double (&x)[8]) { return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])); };
+      // block g's mass of positive values to seg[63 - g], of negative ones to seg[64 + g]: descending order of the values
+#pragma unroll
+      for (int k = 0; k < MINE; ++k) {
+        const int g = wave + kStatWaves * k, m0 = g * 512 + lane * 8;
         double up = 0.0, down = 0.0;
-        if (SPAN == 512 && SPAN * g < INF && pos != 0 && r.top != INFINITY) {
-          const int top_m = (int)pos - 1;
-          const float gap = value(SPAN * g + 1) - value(SPAN * g);
-          const double fall_up = exp2_down(-(double)gap * p.c * (63 - lane)), fall_down = exp2_down(-(double)gap * p.c * lane);
-          // lane k < 8: the largest positive value of the k-th 64; lane 8 + k: the largest negative one
-          const int lead_m = SPAN * g + 64 * (lane & 7) + (lane < 8 ? 63 : 0);
-          const double lead = logit_weight(lane < 8 ? value(lead_m) : -value(lead_m), r.top, p.c);
-#pragma unroll
-          for (int k = 0; k < SPAN / 64; ++k) {
-            const int first = SPAN * g + 64 * k;
-            const bool own = first <= top_m && top_m < first + 63;           // the maximum leads its 64, not the last of them
-            up += plus[k] * (own ? logit_weight(value(first + lane), r.top, p.c) : wave_at(lead, k) * fall_up);
-            down += minus[k] * (wave_at(lead, 8 + k) * fall_down);
-          }
-        } else {
-#pragma unroll
-          for (int k = 0; k < SPAN / 64; ++k) {
-            const float x = value(SPAN * g + 64 * k + lane);
-            up += plus[k] * logit_weight(x, r.top, p.c);
-            down += minus[k] * logit_weight(-x, r.top, p.c);
-          }
+        if (seen[k]) {
+          double mass[8];
+          masses_up(m0, mass);
+          up = wave_scan(sum8(mass));
+          masses_down(m0, mass);
+          down = wave_scan(sum8(mass));
         }
-        up = wave_scan(up);
-        down = wave_scan(down);
-        if (lane == 63) { s.seg[HALF - 1 - g] = up; s.seg[HALF + g] = down; }
+        if (lane == 63) { s.seg[BLOCKS - 1 - g] = up; s.seg[BLOCKS + g] = down; }
       }
       __syncthreads();
-      const double mass = s.seg[tid];                      // zero beyond 2 x HALF
-      const double upto = group_scan<kStatWaves>(mass, s.red);
-      if (tid == kStatThreads - 1) s.found[0] = upto;
-      if (tid == 0) s.key[0] = kStatThreads;
-      __syncthreads();
-      r.z = s.found[0];
-      if (p.top_p < 1.0 && r.top != INFINITY && r.top != -INFINITY) {
-        const double limit = p.top_p * r.z;
-        const unsigned long long past = __builtin_amdgcn_ballot_w64(upto > limit);
-        if (past && lane == 0)
-          __hip_atomic_fetch_min(&s.key[0], (uint32_t)(64 * wave + __builtin_ctzll(past)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        __syncthreads();
-        const uint32_t o = s.key[0];                       // the first group past the limit
-        if ((uint32_t)tid == o) s.found[1] = upto - mass;
-        if (tid == 0) s.key[1] = SPAN;
-        __syncthreads();
-        if (o < 2 * HALF) {
-          // its values in descending order: wave k has the k-th 64 of them, then their masses and those in front
-          const bool positive = o < HALF;
-          const int first = SPAN * (positive ? HALF - 1 - (int)o : (int)o - HALF);
-          double here = 0.0;
-          int m = 0;
-          if (wave < SPAN / 64) {
-            m = positive ? first + SPAN - 1 - 64 * wave - lane : first + 64 * wave + lane;
-            uint32_t plus, minus;
-            weighing(m, plus, minus);
-            here = positive ? plus * logit_weight(value(m), r.top, p.c) : minus * logit_weight(-value(m), r.top, p.c);
-          }
-          double to = wave_scan(here);
-          if (lane == 63) s.red[wave] = to;
-          __syncthreads();
-          to += s.found[1];
-          for (int k = 0; k < wave; ++k) to += s.red[k];
-          if (here > 0.0 && to > limit)
-            __hip_atomic_fetch_min(&s.key[1], (uint32_t)(64 * wave + lane), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-          __syncthreads();
-          // the first value past the limit; where rounding leaves none the whole group stays
-          if ((uint32_t)(64 * wave + lane) == min(s.key[1], (uint32_t)SPAN - 1)) {
-            s.found[0] = to;
-            s.redu[0][0] = __float_as_uint(positive ? value(m) : -value(m));
-          }
-          __syncthreads();
-          r.z = s.found[0];
-          r.cut = __uint_as_float(s.redu[0][0]);
+      // every wave: the block past which the mass exceeds top_p of all
+      const double first = s.seg[2 * lane], second = s.seg[2 * lane + 1];
+      const double upto = wave_scan(first + second);
+      const double z = wave_at(upto, 63), limit = p.top_p * z;
+      const unsigned long long past = p.top_p < 1.0 ? __builtin_amdgcn_ballot_w64(upto > limit) : 0;
+      if (!past) {                                         // everything stays
+        if (tid == 0) { p.z[at] = z; p.top[at] = top; p.cut[at] = -INFINITY; }
+        return;
+      }
+      const int l = __builtin_ctzll(past);
+      double above = wave_at(upto, l) - wave_at(first, l) - wave_at(second, l);
+      int o = 2 * l;
+      if (above + wave_at(first, l) <= limit) { above += wave_at(first, l); ++o; }
+      const bool positive = o < BLOCKS;
+      const int g = positive ? BLOCKS - 1 - o : o - BLOCKS;
+      if (g % kStatWaves != wave) return;
+      // the wave that holds the block: its masses in descending order, lanes from 63 down for positive values
+      double mass[8];
+      const int m0 = g * 512 + lane * 8;
+      if (positive) masses_up(m0, mass);
+      else masses_down(m0, mass);
+      const double own = sum8(mass), scan = wave_scan(own);
+      double run = above + (positive ? wave_at(scan, 63) - scan : scan - own);       // mass above this lane's values
+      int cross = 8, some = -1;
+      double kept = 0.0, kept_some = 0.0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        run += mass[j];
+        if (mass[j] > 0.0) {
+          some = j;
+          kept_some = run;
+          if (cross == 8 && run > limit) { cross = j; kept = run; }
         }
       }
+      const unsigned long long hit = __builtin_amdgcn_ballot_w64(cross < 8), any = __builtin_amdgcn_ballot_w64(some >= 0);
+      // the first value past the limit; where rounding leaves none, the block's last
+      const int who = hit ? (positive ? 63 - __builtin_clzll(hit) : __builtin_ctzll(hit))
+                          : (positive ? __builtin_ctzll(any | 1ull << 63) : 63 - __builtin_clzll(any | 1ull));
+      if (lane == who) {
+        const int j = hit ? cross : max(some, 0);
+        p.z[at] = hit ? kept : some >= 0 ? kept_some : run;
+        p.top[at] = top;
+        p.cut[at] = positive ? value(m0 + 7 - j) : -value(m0 + j);
+      }
+      return;
     }
   }
-  if (!counted) {
-    __syncthreads();
-    r = search_row<DT>(ptr, p, (uint64_t*)lds_raw, s);
-  }
+  __syncthreads();
+  const RowStats r = search_row<DT>(ptr, p, (uint64_t*)lds_raw, s);
   if (tid == 0) {
     p.z[at] = r.z;
     p.top[at] = r.top;
@@ -871,7 +910,7 @@ extern "C" int pa_verify_drafts(const void* logits, int dtype, int64_t row_strid
   p.chunks = (int)((vocab + kChunk - 1) / kChunk);
   // as many workgroups of the second launch as the GPU holds at once (six per CU): a wave's chunks are a chain of loads and
   // sums, so fewer of them each (512 workgroups: 32 us for 64 rows of 152k entries with draft probabilities)
-  const int64_t want = (1536 + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
+  const int64_t want = ((p.q ? 1536 : 768) + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
   p.slices = (int)(want < most ? want : most);
   p.z = (double*)(ws + l.z);
   p.top = (float*)(ws + l.top);

@@ -4,10 +4,11 @@
 // entry's argument kinds once (bind), and then calls by index (call).  Nothing is computed here.
 //
 // Calling convention (x86-64 System V): pointer and integer arguments travel in the integer
-// registers and then on the stack, in order; float arguments in the vector registers, in order;
+// registers and then on the stack, in order; floating arguments in the vector registers, in order;
 // the two sequences do not interact.  So an entry point `int f(void*, int, long, float, void*)`
-// can be called as `f(long, long, long, long, float)`: the integer-class arguments first, widened
-// to 64 bits (a callee that takes an `int` reads the low half), then the floats.  Arguments beyond
+// can be called as `f(long, long, long, long, double)`: the integer-class arguments first, widened
+// to 64 bits (a callee that takes an `int` reads the low half), then the floating ones, a float's bits in
+// the low half of a double's (a callee that takes a `float` reads that half).  Arguments beyond
 // those the callee takes are ignored by it (the caller owns the stack), which lets one call site
 // with a fixed number of slots serve every signature.
 #define PY_SSIZE_T_CLEAN
@@ -22,7 +23,7 @@
 
 typedef struct {
   void* fn;
-  char kinds[MAX_INTS + MAX_FLOATS + 1];  // per argument: p pointer (None = null), q int64, i int, f float
+  char kinds[MAX_INTS + MAX_FLOATS + 1];  // per argument: p pointer (None = null), q int64, i int, f float, d double
   int nargs;
   int wide;  // the entry returns int64 instead of int
 } Bound;
@@ -32,7 +33,7 @@ static int g_nbound = 0;
 
 typedef int64_t L;
 typedef L (*Entry)(L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L, L,
-                   L, L, L, L, L, L, float, float);
+                   L, L, L, L, L, L, double, double);
 
 // bind(address, kinds, returns_int64) -> index
 static PyObject* fc_bind(PyObject* self, PyObject* args) {
@@ -43,10 +44,10 @@ static PyObject* fc_bind(PyObject* self, PyObject* args) {
   const size_t n = strlen(kinds);
   int ints = 0, floats = 0;
   for (size_t k = 0; k < n; ++k) {
-    if (kinds[k] == 'f') ++floats;
+    if (kinds[k] == 'f' || kinds[k] == 'd') ++floats;
     else if (kinds[k] == 'p' || kinds[k] == 'q' || kinds[k] == 'i') ++ints;
     else {
-      PyErr_SetString(PyExc_ValueError, "pa_fastcall.bind: argument kinds are p, q, i and f");
+      PyErr_SetString(PyExc_ValueError, "pa_fastcall.bind: argument kinds are p, q, i, f and d");
       return NULL;
     }
   }
@@ -79,7 +80,7 @@ static PyObject* fc_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
     return NULL;
   }
   L a[MAX_INTS];
-  float f[MAX_FLOATS] = {0.0f, 0.0f};
+  double f[MAX_FLOATS] = {0.0, 0.0};
   memset(a, 0, sizeof(a));
   int ni = 0, nf = 0;
   for (int k = 0; k < b->nargs; ++k) {
@@ -112,10 +113,15 @@ static PyObject* fc_call(PyObject* self, PyObject* const* args, Py_ssize_t nargs
         a[ni++] = (L)v;
         break;
       }
-      default: {  // 'f'
+      default: {  // 'f' or 'd'
         const double v = PyFloat_AsDouble(o);
         if (v == -1.0 && PyErr_Occurred()) return NULL;
-        f[nf++] = (float)v;
+        if (b->kinds[k] == 'd') {
+          f[nf++] = v;
+        } else {
+          const float single = (float)v;
+          memcpy(&f[nf++], &single, sizeof(single));
+        }
         break;
       }
     }

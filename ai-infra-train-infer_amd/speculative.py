@@ -30,6 +30,16 @@ MAX_DRAFT_NODES = 256
 _get_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(batch, nodes, num_q_heads, head_dim, parts):
+    return _native.load().pa_draft_workspace_bytes(batch, nodes, num_q_heads, head_dim, parts)
+
+
+@functools.lru_cache(maxsize=1024)
+def _verify_workspace(batch, nodes, vocab):
+    return _native.load().pa_verify_workspace_bytes(batch, nodes, vocab)
+
+
 def _same_device(what, first, *others):
     """Launches go to the current device: every tensor has to be there."""
     for t in others:
@@ -225,7 +235,7 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
         parts = max(1, -(-tables.shape[1] * block_size // psize)) if psize > 0 else 1
     ws_ptr, ws_bytes = None, 0
     if parts > 1:
-        ws_bytes = lib.pa_draft_workspace_bytes(batch, nodes, num_q_heads, head_dim, parts)
+        ws_bytes = _attention_workspace(batch, nodes, num_q_heads, head_dim, parts)
         if workspace is not None:
             if workspace.dtype != torch.uint8 or workspace.numel() < ws_bytes or not workspace.is_contiguous():
                 raise RuntimeError("%s: workspace must be a contiguous uint8 GPU tensor of at least %d bytes" % (what, ws_bytes))
@@ -301,7 +311,7 @@ def verify_drafts(logits, draft_tokens, uniforms=None, parents=None, num_nodes=N
             probs = draft_probs
             if probs.stride(2) != 1 or (nodes > 2 and probs.stride(1) < vocab) or (batch > 1 and probs.stride(0) < vocab):
                 probs = probs.contiguous()
-    ws_bytes = lib.pa_verify_workspace_bytes(batch, nodes, vocab)
+    ws_bytes = _verify_workspace(batch, nodes, vocab)
     if workspace is None:
         workspace = reserve_decode_workspace(device, ws_bytes)
     elif workspace.dtype != torch.uint8 or workspace.numel() < ws_bytes or not workspace.is_contiguous():

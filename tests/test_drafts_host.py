@@ -90,6 +90,18 @@ def test_layout_c_abi_refusals(lib):
     assert call(nodes=257, stride=257) == -2 and call(blocks=1 << 28) == -2
 
 
+def test_fast_bindings_pass_doubles_and_floats(lib):
+    """pa_verify_drafts takes two doubles, pa_draft_attention one float: the quick binding and ctypes agree on what the entry
+    sees, tested through refusals that depend on the value."""
+    need = lib.pa_verify_workspace_bytes(2, 5, 1000)
+    for temperature, top_p, want in ((1e-7, 0.5, -2), (1.0, 0.0, -1), (0.5, -1.0, -1), (1e7, 0.5, -2), (float("nan"), 0.5, -1), (1, 0, -1)):
+        args = (P, 0, 1000, 5000, P, P, None, 0, None, None, 2, 1000, 4000, temperature, top_p, 2, 5, 1000, P, P, P, P, need, None)
+        assert lib.pa_verify_drafts(*args) == lib._cdll.pa_verify_drafts(*args) == want, (temperature, top_p)
+    for scale in (0.0, -1.0, float("inf"), float("nan")):
+        args = (P, 0, 2048, P, P, None, None, 0, P, 8, 8, P, None, P, 5, P, 2048, 2, 5, 16, 8, 128, 16, 100, scale, 64, 1, None, 0, 0, None)
+        assert lib.pa_draft_attention(*args) == lib._cdll.pa_draft_attention(*args) == -1
+
+
 def test_verify_c_abi_refusals(lib):
     need = lib.pa_verify_workspace_bytes(2, 5, 1000)
     assert need > 0 and lib.pa_verify_workspace_bytes(0, 5, 10) == 0
