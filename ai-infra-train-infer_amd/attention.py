@@ -1199,6 +1199,8 @@ class PagedAttention(nn.Module):
                            cache_dtype=self.cache_dtype)
         if ctx.is_prefill:
             return self._prefill_attention(q, k, v, ctx)
+        if ctx.tree_mask is not None:
+            return self._draft_attention(q, ctx)
         return self._decode_attention(q, ctx)
 
     def forward_fused(self, q, k, v, q_norm_weight, k_norm_weight, eps, inv_freq, positions):
@@ -1214,6 +1216,8 @@ class PagedAttention(nn.Module):
             cache_dtype=self.cache_dtype, return_k=dense_k)
         if ctx.is_prefill:
             return self._prefill_attention(q, k_rot, v, ctx)
+        if ctx.tree_mask is not None:
+            return self._draft_attention(q, ctx)
         return self._decode_attention(q, ctx)
 
     def _scales(self):
@@ -1229,6 +1233,17 @@ class PagedAttention(nn.Module):
                                  k_scale=ks, v_scale=vs)
         return paged_prefill(q, k, v, ctx.cu_seqlens_q, ctx.cu_seqlens_k, ctx.max_seqlen_q,
                              self.scale)
+
+    def _draft_attention(self, q, ctx):
+        """A step that checks drafted tokens: every row's tree_mask.shape[1] nodes against its committed tokens and
+        their own ancestors (speculative.paged_draft_attention)."""
+        from .speculative import paged_draft_attention
+        if self.k_cache is None or ctx.block_tables is None or ctx.context_lens is None:
+            return q
+        ks, vs = self._scales()
+        return paged_draft_attention(q, self.k_cache, self.v_cache, ctx.block_tables, ctx.context_lens, ctx.tree_mask,
+                                     self.scale, k_scale=ks, v_scale=vs, num_nodes=ctx.num_nodes,
+                                     longest_context=ctx.longest_context_len or None, mean_context=ctx.mean_context_len or None)
 
     def _decode_attention(self, q, ctx):
         if self.k_cache is None or ctx.block_tables is None or ctx.context_lens is None:

@@ -35,6 +35,11 @@ class InferenceContext:
     # instead of for the width of the block table (attention.choose_partition); 0 = unknown
     longest_context_len: int = 0
     mean_context_len: float = 0.0
+    # a step that checks drafted tokens (no counterpart in the reference): which nodes each node sees, as
+    # speculative.draft_layout() returns it, and how many nodes each row drafts (None: all); context_lens
+    # then counts the committed tokens only, and every row has tree_mask.shape[1] tokens in the forward
+    tree_mask: Optional[torch.Tensor] = None
+    num_nodes: Optional[torch.Tensor] = None
 
 
 _CONTEXT = InferenceContext()
@@ -52,6 +57,8 @@ def set_context(
     prefix_groups: Optional[object] = None,
     longest_context_len: int = 0,
     mean_context_len: float = 0.0,
+    tree_mask: Optional[torch.Tensor] = None,
+    num_nodes: Optional[torch.Tensor] = None,
 ):
     """Install the context for the next model forward."""
     global _CONTEXT
@@ -67,6 +74,8 @@ def set_context(
         prefix_groups=prefix_groups,
         longest_context_len=longest_context_len,
         mean_context_len=mean_context_len,
+        tree_mask=tree_mask,
+        num_nodes=num_nodes,
     )
 
 

@@ -152,6 +152,12 @@ class BlockPool:
                 raise RuntimeError("pa_copy_blocks failed (%d): %s"
                                    % (rc, lib.pa_last_error().decode("utf-8", "replace")))
 
+    def commit_drafts(self, block_tables, context_lens, path, counts):
+        """Move the kept nodes of a speculative step to consecutive positions, in all layers, K, V and fp8 scales
+        (speculative.commit_drafts); returns the new context_lens."""
+        from .speculative import commit_drafts
+        return commit_drafts(self._kv_cache, block_tables, context_lens, path, counts, self.k_scale, self.v_scale)
+
     # ---------------------------------------------------------------- device tensors
 
     def _allocate_gpu_memory(self):

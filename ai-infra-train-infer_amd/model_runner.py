@@ -745,6 +745,26 @@ class ModelRunner:
         set_context(is_prefill=False, slot_mapping=slots, context_lens=context_lens, block_tables=block_tables)
         return self.run(input_ids, positions, is_prefill=False)
 
+    @torch.inference_mode()
+    def run_drafts(self, tokens, parents, block_tables, context_lens, num_nodes=None, longest_context=0, mean_context=0.0):
+        """The target's forward over the drafted nodes of a batch (speculative.py): tokens int64 [batch, nodes] (node 0:
+        the last accepted token), parents int32 [nodes] or [batch, nodes], block_tables [batch, max_blocks] int32 that
+        reach context_len + nodes, context_lens [batch] int32 (committed tokens), num_nodes int32 [batch] or None ->
+        logits [batch, nodes, vocab], the distribution after every node.  Node i's K and V are written at cache
+        position context_len + i of every layer.  longest_context / mean_context: what the host knows of context_lens."""
+        from .speculative import draft_layout
+        if self.model is None:
+            raise RuntimeError("run_drafts: the runner has no model of PagedAttention layers")
+        num_blocks = self._kv_cache.shape[2] if self._kv_cache is not None else 2 ** 31 // self.block_size - 1
+        positions, slots, mask = draft_layout(parents, context_lens, block_tables, self.block_size, num_blocks, num_nodes)
+        set_context(is_prefill=False, slot_mapping=slots.view(-1), context_lens=context_lens, block_tables=block_tables,
+                    longest_context_len=longest_context, mean_context_len=mean_context, tree_mask=mask, num_nodes=num_nodes)
+        try:
+            logits = self.model(tokens.reshape(-1), positions=positions.view(-1))
+        finally:
+            reset_context()
+        return logits.view(*tokens.shape, -1)
+
     # ---------------------------------------------------------------- HuggingFace-style models
     # The reference's shipped kv_cache mode (src/inference/model_runner.py:118-462): the model is
     # a HuggingFace causal LM that knows nothing of paging; its K/V are written into the paged pool

@@ -14,10 +14,10 @@ they are to be tried.  A step:
 
 ModelRunner.run_drafts() is the middle line for a model of PagedAttention layers.  context_lens counts the committed
 tokens throughout; num_nodes (int32 [batch]) says how many nodes a row really drafts, 0 for a padded row.  Nothing
-here synchronises with the host, so a step can be recorded in a HIP graph.
+here synchronises with the host, so a step can be recorded in a HIP graph (after a warm-up run inside
+attention.sizing_graph_workspace(), as for paged_decode; graphs that replay at the same time need workspaces of their own).
 """
 import functools
-
 
 import torch
 
@@ -337,7 +337,8 @@ def commit_drafts(kv_cache, block_tables, context_lens, path, counts, k_scale=No
     kv_cache [2, layers, num_blocks, block_size, kv_heads, head_dim], contiguous (BlockPool.kv_cache_tensor), changed in
     place; k_scale / v_scale [layers, num_blocks, block_size] of an fp8 pool, changed with it.  path and counts as
     verify_drafts returns them.  The blocks that hold the drafted positions must be the row's own (a shared last block
-    is copied before it is written, as for any decode step)."""
+    is copied before it is written, as for any decode step); those behind the next token's are free again, and have to
+    leave a row's table before ModelRunner.prepare_decode() sees it."""
     what = "commit_drafts"
     _require_gpu(kv_cache, what)
     if kv_cache.dim() != 6 or kv_cache.shape[0] != 2 or not kv_cache.is_contiguous():

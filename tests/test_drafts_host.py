@@ -155,3 +155,31 @@ def test_attention_c_abi_refusals(lib):
                 dict(batch=65536), dict(hq=65536, hkv=8, qs=1 << 30, os=1 << 30)):
         assert call(**{**bad, "ws_bytes": 1 << 50}) == -2, bad
     assert call(ws=None) == -4 and call(ws_bytes=need - 1) == -4
+
+
+def test_attention_launch_policy(pa):
+    from ai_infra_train_infer_amd.speculative import _choose_draft_launch as choose
+    for batch in (1, 3, 64, 400):
+        for nodes in (1, 5, 33, 256):
+            for heads, kv_heads in ((1, 1), (16, 8), (24, 3), (64, 8)):
+                for keys in (1, 16, 127, 1000, 40000, 1 << 20):
+                    for mean in {max(1, keys // 16), keys}:
+                        tile, size, parts = choose(batch, nodes, heads, kv_heads, 128, 2, keys, mean, 256)
+                        assert tile in (16, 32, 64, 128) and 1 <= parts <= 64
+                        if parts == 1:
+                            assert size == 0
+                        else:       # the partitions cover every key, the last one at least one of them
+                            assert size % 32 == 0 and (parts - 1) * size < keys <= parts * size
+    # a lone sequence of 32k tokens is split over the chip, a batch that fills it is not
+    assert choose(1, 5, 16, 8, 128, 2, 32768, 32768, 256)[2] > 8
+    assert choose(256, 5, 16, 8, 128, 2, 512, 512, 256)[2] == 1
+    # narrow tiles for chains, wide ones where many rows share the keys
+    assert choose(1, 5, 16, 8, 128, 2, 4096, 4096, 256)[0] == 16
+    assert choose(32, 64, 16, 8, 128, 2, 4096, 4096, 256)[0] == 128
+
+
+def test_run_drafts_refuses_a_runner_without_a_model(pa):
+    runner = pa.ModelRunner(None, pa.ModelRunnerConfig(block_size=16, device="cpu"))
+    one = torch.zeros(1, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="no model"):
+        runner.run_drafts(one.long(), one, one, one[0])
