@@ -41,20 +41,30 @@ def _verify_workspace(batch, nodes, vocab):
 
 
 def _same_device(what, first, *others):
-    """Launches go to the current device: every tensor has to be there."""
+    """Launches go to the current device, whose index this returns: every tensor has to be there."""
+    index = first.get_device()
+    if index < 0:
+        _require_gpu(first, what)
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise RuntimeError("%s: tensors on %s and %s" % (what, first.device, t.device))
-    if first.device.index != _get_device():
+    if index != _get_device():
         raise RuntimeError("%s: the tensors are on %s, the current device is cuda:%d (use torch.cuda.device)"
                            % (what, first.device, _get_device()))
+    return index
 
 
 def _tables(block_tables, batch, what):
-    if block_tables.dim() != 2 or block_tables.shape[0] != batch:
+    """(int32 tensor, stride between rows, columns)"""
+    shape = block_tables.shape
+    if len(shape) != 2 or shape[0] != batch:
         raise RuntimeError("%s: block_tables must be [batch, max_blocks]" % what)
-    tables = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
-    return tables if tables.stride(1) == 1 and tables.stride(0) >= tables.shape[1] else tables.contiguous()
+    if block_tables.dtype != torch.int32:
+        block_tables = block_tables.to(torch.int32)
+    row, column = block_tables.stride()
+    if column != 1 or row < shape[1]:
+        block_tables, row = block_tables.contiguous(), shape[1]
+    return block_tables, row, shape[1]
 
 
 def _lengths(t, batch, name, what):
@@ -68,9 +78,10 @@ def _lengths(t, batch, name, what):
 def _trees(parents, batch, nodes, what):
     """(int32 tensor, stride between rows): stride 0 for one tree that every row drafts."""
     parents = _int32(parents, what)
-    if parents.dim() == 1 and parents.shape[0] == nodes:
+    shape = parents.shape
+    if len(shape) == 1 and shape[0] == nodes:
         return parents, 0
-    if tuple(parents.shape) != (batch, nodes):
+    if shape != (batch, nodes):
         raise RuntimeError("%s: parents must be [nodes] or [batch, nodes]" % what)
     return parents, nodes
 
@@ -85,10 +96,9 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
     writers skip, as do nodes whose position lies outside the block table or the pool.  Bit j % 64 of word j / 64 of a
     mask row is set where node j is the node itself or one of its ancestors."""
     what = "draft_layout"
-    _require_gpu(context_lens, what)
-    _same_device(what, context_lens, parents, block_tables, num_nodes)
+    device = _same_device(what, context_lens, parents, block_tables, num_nodes)
     lib = _native.load()
-    lens = _int32(context_lens, what).reshape(-1)
+    lens = _int32(context_lens, what)
     batch = lens.numel()
     if parents.dim() not in (1, 2):
         raise RuntimeError("%s: parents must be [nodes] or [batch, nodes]" % what)
@@ -97,22 +107,21 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
         raise RuntimeError("%s: a row drafts 1 to %d nodes, got %d" % (what, MAX_DRAFT_NODES, nodes))
     parents, stride = _trees(parents, batch, nodes, what)
     real = _lengths(num_nodes, batch, "num_nodes", what)
-    device = lens.device
-    positions = torch.empty((batch, nodes), dtype=torch.int64, device=device)
-    mask = torch.empty((batch if stride else 1, nodes, (nodes + 63) // 64), dtype=torch.int64, device=device)
-    slots = tables = None
+    positions = lens.new_empty((batch, nodes), dtype=torch.int64)
+    mask = positions.new_empty((batch if stride else 1, nodes, (nodes + 63) // 64))
+    slots = tables = tables_ptr = slots_ptr = None
+    row = width = 0
     if block_tables is not None:
         if num_blocks is None:
             raise RuntimeError("%s: num_blocks is needed with block_tables" % what)
-        tables = _tables(block_tables, batch, what)
-        slots = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+        tables, row, width = _tables(block_tables, batch, what)
+        slots = lens.new_empty((batch, nodes))
+        tables_ptr, slots_ptr = tables.data_ptr(), slots.data_ptr()
     if batch == 0:
         return positions, slots, mask
     rc = lib.pa_draft_layout(parents.data_ptr(), stride, lens.data_ptr(), real.data_ptr() if real is not None else None,
-                             tables.data_ptr() if tables is not None else None, tables.stride(0) if tables is not None else 0,
-                             tables.shape[1] if tables is not None else 0, positions.data_ptr(),
-                             slots.data_ptr() if slots is not None else None, mask.data_ptr(), batch, nodes, int(block_size),
-                             int(num_blocks or 1), _stream_ptr(device))
+                             tables_ptr, row, width, positions.data_ptr(), slots_ptr, mask.data_ptr(), batch, nodes,
+                             int(block_size), int(num_blocks or 1), _stream_ptr(device))
     _native.check(rc, "pa_draft_layout")
     return positions, slots, mask
 
@@ -180,50 +189,59 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
     the device's shared one.  longest_context / mean_context: what the host knows about context_lens, as for paged_decode;
     wrong values cost time, never correctness."""
     what = "paged_draft_attention"
-    _require_gpu(q, what)
-    _require_gpu(k_cache, what)
+    device = _same_device(what, q, k_cache, v_cache, block_tables, context_lens, tree_mask, k_scale, v_scale, num_nodes, out,
+                          workspace)
     _check_cache(k_cache, v_cache, what)
-    _same_device(what, q, k_cache, v_cache, block_tables, context_lens, tree_mask, k_scale, v_scale, num_nodes, out, workspace)
     lib = _native.load()
     batch = context_lens.numel()
-    if tree_mask.dim() != 3 or tree_mask.dtype != torch.int64 or tree_mask.shape[0] not in (1, batch):
+    masks = tree_mask.shape
+    if len(masks) != 3 or tree_mask.dtype != torch.int64 or masks[0] not in (1, batch):
         raise RuntimeError("%s: tree_mask must be int64 [batch or 1, nodes, words]" % what)
-    nodes = tree_mask.shape[1]
-    if not 1 <= nodes <= MAX_DRAFT_NODES or tree_mask.shape[2] != (nodes + 63) // 64:
-        raise RuntimeError("%s: tree_mask %s is not one of 1 to %d nodes" % (what, tuple(tree_mask.shape), MAX_DRAFT_NODES))
-    if q.dim() not in (3, 4) or q.shape[:-2].numel() != batch * nodes or (q.dim() == 4 and q.shape[1] != nodes):
-        raise RuntimeError("%s: q %s does not match %d rows of %d nodes" % (what, tuple(q.shape), batch, nodes))
-    num_q_heads, head_dim = q.shape[-2:]
+    nodes = masks[1]
+    if not 1 <= nodes <= MAX_DRAFT_NODES or masks[2] != (nodes + 63) // 64:
+        raise RuntimeError("%s: tree_mask %s is not one of 1 to %d nodes" % (what, tuple(masks), MAX_DRAFT_NODES))
+    shape = q.shape
+    if (shape[:2] != (batch, nodes)) if len(shape) == 4 else (len(shape) != 3 or shape[0] != batch * nodes):
+        raise RuntimeError("%s: q %s does not match %d rows of %d nodes" % (what, tuple(shape), batch, nodes))
+    num_q_heads, head_dim = shape[-2:]
     num_blocks, block_size, num_kv_heads, d2 = k_cache.shape
     if d2 != head_dim:
         raise RuntimeError("%s: q head_dim %d != cache head_dim %d" % (what, head_dim, d2))
-    flat = q if q.dim() == 3 else q.reshape(batch * nodes, num_q_heads, head_dim)
-    if (flat.stride(2) != 1 or flat.stride(1) != head_dim or flat.data_ptr() % 16 or flat.stride(0) * flat.element_size() % 16
-            or (flat.shape[0] > 1 and flat.stride(0) < num_q_heads * head_dim)):
-        flat = flat.contiguous()
-    tables = _tables(block_tables, batch, what)
+    flat, q_stride, dense = q, num_q_heads * head_dim, q.is_contiguous()
+    if not dense:
+        flat = q if len(shape) == 3 else q.reshape(batch * nodes, num_q_heads, head_dim)
+        if (flat.stride(2) != 1 or flat.stride(1) != head_dim or flat.stride(0) * flat.element_size() % 16
+                or (flat.shape[0] > 1 and flat.stride(0) < q_stride)):
+            flat = flat.contiguous()
+        elif flat.shape[0] > 1:
+            q_stride = flat.stride(0)
+    if flat.data_ptr() % 16:
+        flat, q_stride = flat.clone(memory_format=torch.contiguous_format), num_q_heads * head_dim
+    tables, tables_row, width = _tables(block_tables, batch, what)
     lens = _int32(context_lens, what)
     real = _lengths(num_nodes, batch, "num_nodes", what)
     mask = tree_mask.contiguous()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if dense else torch.empty(shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise RuntimeError("%s: out must be contiguous and like q" % what)
     if batch == 0:
         return out
     kv_code = _code(k_cache.dtype, what)
+    scales = (None, None)
     fp8 = kv_code == _native.DTYPE_FP8_E4M3
     if fp8:
         for t in (k_scale, v_scale):
             if t is None or t.dtype != torch.float32 or t.numel() != num_blocks * block_size or not t.is_contiguous():
                 raise RuntimeError("%s: an fp8 cache needs contiguous fp32 k_scale and v_scale [num_blocks, block_size]" % what)
+        scales = (k_scale.data_ptr(), v_scale.data_ptr())
     if _debug_tables():
         bad, short = check_block_tables(tables, lens + (real if real is not None else nodes), block_size, num_blocks)
         if bad or short:
             raise RuntimeError("%s: %d block-table entries outside the pool of %d blocks, %d rows whose tokens need more "
-                               "than the table's %d columns" % (what, bad, num_blocks, short, tables.shape[1]))
+                               "than the table's %d columns" % (what, bad, num_blocks, short, width))
     if partition_size is None:
-        bound = tables.shape[1] * block_size
+        bound = width * block_size
         if longest_context:
             bound = min(bound, -(-(int(longest_context) + nodes) // 256) * 256)
         # sixteenths of the bound: batches of about the same shape share the decision
@@ -232,7 +250,7 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
                                                   bound, mean, _compute_units(q.device))
     else:
         tile, psize = 0, int(partition_size)
-        parts = max(1, -(-tables.shape[1] * block_size // psize)) if psize > 0 else 1
+        parts = max(1, -(-width * block_size // psize)) if psize > 0 else 1
     ws_ptr, ws_bytes = None, 0
     if parts > 1:
         ws_bytes = _attention_workspace(batch, nodes, num_q_heads, head_dim, parts)
@@ -243,13 +261,12 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
         else:
             ws = reserve_decode_workspace(q.device, ws_bytes)
         ws_ptr = ws.data_ptr()
-    rc = lib.pa_draft_attention(flat.data_ptr(), _code(flat.dtype, what), flat.stride(0) if flat.shape[0] > 1 else num_q_heads * head_dim,
-                                k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr() if fp8 else None,
-                                v_scale.data_ptr() if fp8 else None, kv_code, tables.data_ptr(), tables.stride(0),
-                                tables.shape[1], lens.data_ptr(), real.data_ptr() if real is not None else None,
-                                mask.data_ptr(), mask.shape[1] * mask.shape[2] if mask.shape[0] > 1 else 0, out.data_ptr(),
-                                num_q_heads * head_dim, batch, nodes, num_q_heads, num_kv_heads, head_dim, block_size,
-                                num_blocks, float(scale), psize, parts, ws_ptr, ws_bytes, tile, _stream_ptr(q.device))
+    rc = lib.pa_draft_attention(flat.data_ptr(), _code(q.dtype, what), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), *scales,
+                                kv_code, tables.data_ptr(), tables_row, width, lens.data_ptr(),
+                                real.data_ptr() if real is not None else None, mask.data_ptr(),
+                                nodes * masks[2] if masks[0] > 1 else 0, out.data_ptr(), num_q_heads * head_dim, batch, nodes,
+                                num_q_heads, num_kv_heads, head_dim, block_size, num_blocks, float(scale), psize, parts, ws_ptr,
+                                ws_bytes, tile, _stream_ptr(device))
     _native.check(rc, "pa_draft_attention")
     return out
 
@@ -271,24 +288,24 @@ def verify_drafts(logits, draft_tokens, uniforms=None, parents=None, num_nodes=N
     certain and accepted with the target's probability, siblings one after the other with what the earlier ones leave.
     Either way the emitted tokens are distributed as the target's own samples."""
     what = "verify_drafts"
-    _require_gpu(logits, what)
+    index = _same_device(what, logits, draft_tokens, uniforms, parents, num_nodes, draft_probs, workspace)
     if logits.dim() != 3:
         raise RuntimeError("%s: logits must be [batch, nodes, vocab], got %s" % (what, tuple(logits.shape)))
     batch, nodes, vocab = logits.shape
-    _same_device(what, logits, draft_tokens, uniforms, parents, num_nodes, draft_probs, workspace)
     if not 1 <= nodes <= MAX_DRAFT_NODES:
         raise RuntimeError("%s: a row drafts 1 to %d nodes, got %d" % (what, MAX_DRAFT_NODES, nodes))
-    if tuple(draft_tokens.shape) != (batch, nodes) or draft_tokens.dtype != torch.int64:
+    if draft_tokens.shape != (batch, nodes) or draft_tokens.dtype != torch.int64:
         raise RuntimeError("%s: draft_tokens must be int64 [batch, nodes]" % what)
     lib = _native.load()
     temperature, top_p = float(temperature), float(top_p)
     device = logits.device
-    if logits.stride(2) != 1 or (nodes > 1 and logits.stride(1) < vocab) or (batch > 1 and logits.stride(0) < vocab):
+    if not logits.is_contiguous() and (logits.stride(2) != 1 or (nodes > 1 and logits.stride(1) < vocab)
+                                       or (batch > 1 and logits.stride(0) < vocab)):
         logits = logits.contiguous()
     tokens = draft_tokens.contiguous()
-    tokens_out = torch.empty((batch, nodes), dtype=torch.int64, device=device)
+    tokens_out = torch.empty_like(tokens)
     counts = torch.empty(batch, dtype=torch.int32, device=device)
-    path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
+    path = counts.new_empty((batch, nodes))
     if batch == 0:
         return tokens_out, counts, path
     stride = 0
@@ -298,14 +315,14 @@ def verify_drafts(logits, draft_tokens, uniforms=None, parents=None, num_nodes=N
     if temperature > 0:
         if uniforms is None:
             uniforms = torch.rand((batch, nodes), device=device, dtype=torch.float32, generator=generator)
-        if tuple(uniforms.shape) != (batch, nodes) or uniforms.dtype != torch.float32:
+        if uniforms.shape != (batch, nodes) or uniforms.dtype != torch.float32:
             raise RuntimeError("%s: uniforms must be fp32 [batch, nodes]" % what)
         uniforms = uniforms.contiguous()
     probs = None
     if draft_probs is not None:
         if parents is not None:
             raise RuntimeError("%s: draft_probs go with chains (parents=None) only" % what)
-        if tuple(draft_probs.shape) != (batch, nodes - 1, vocab):
+        if draft_probs.shape != (batch, nodes - 1, vocab):
             raise RuntimeError("%s: draft_probs must be [batch, nodes - 1, vocab], got %s" % (what, tuple(draft_probs.shape)))
         if nodes > 1 and temperature > 0:
             probs = draft_probs
@@ -325,7 +342,7 @@ def verify_drafts(logits, draft_tokens, uniforms=None, parents=None, num_nodes=N
                               (probs.stride(1) if nodes > 2 else vocab) if probs is not None else 0,
                               (probs.stride(0) if batch > 1 else 0) if probs is not None else 0, temperature, top_p,
                               batch, nodes, vocab, tokens_out.data_ptr(), counts.data_ptr(), path.data_ptr(),
-                              workspace.data_ptr(), ws_bytes, _stream_ptr(device))
+                              workspace.data_ptr(), ws_bytes, _stream_ptr(index))
     _native.check(rc, "pa_verify_drafts")
     return tokens_out, counts, path
 
@@ -340,33 +357,34 @@ def commit_drafts(kv_cache, block_tables, context_lens, path, counts, k_scale=No
     is copied before it is written, as for any decode step); those behind the next token's are free again, and have to
     leave a row's table before ModelRunner.prepare_decode() sees it."""
     what = "commit_drafts"
-    _require_gpu(kv_cache, what)
+    device = _same_device(what, kv_cache, block_tables, context_lens, path, counts, k_scale, v_scale)
     if kv_cache.dim() != 6 or kv_cache.shape[0] != 2 or not kv_cache.is_contiguous():
         raise RuntimeError("%s: kv_cache must be contiguous [2, layers, num_blocks, block_size, kv_heads, head_dim]" % what)
-    _same_device(what, kv_cache, block_tables, context_lens, path, counts, k_scale, v_scale)
     lib = _native.load()
     _, layers, num_blocks, block_size, heads, head_dim = kv_cache.shape
-    lens = _int32(context_lens, what).reshape(-1)
+    lens = _int32(context_lens, what)
+    if lens.dim() != 1:
+        lens = lens.view(-1)
     batch = lens.numel()
     if path.dim() != 2 or path.shape[0] != batch or path.shape[1] > MAX_DRAFT_NODES:
         raise RuntimeError("%s: path must be [batch, nodes] of at most %d nodes" % (what, MAX_DRAFT_NODES))
     path = _int32(path, what)
     counts = _lengths(counts, batch, "counts", what)
-    tables = _tables(block_tables, batch, what)
+    tables, tables_row, width = _tables(block_tables, batch, what)
     es = kv_cache.element_size()
     fp8 = es == 1
     if fp8:
         for t in (k_scale, v_scale):
             if t is None or t.dtype != torch.float32 or t.numel() != layers * num_blocks * block_size or not t.is_contiguous():
                 raise RuntimeError("%s: an fp8 pool needs contiguous fp32 k_scale and v_scale [layers, num_blocks, block_size]" % what)
-    new_lens = torch.empty(batch, dtype=torch.int32, device=kv_cache.device)
+    new_lens = torch.empty_like(lens)
     if batch == 0:
         return new_lens
     row = heads * head_dim * es
     rc = lib.pa_draft_commit(kv_cache.data_ptr(), layers, num_blocks * block_size * row, row,
                              k_scale.data_ptr() if fp8 else None, v_scale.data_ptr() if fp8 else None, num_blocks * block_size,
-                             tables.data_ptr(), tables.stride(0), tables.shape[1], lens.data_ptr(), path.data_ptr(),
-                             path.shape[1], counts.data_ptr(), new_lens.data_ptr(), batch, path.shape[1], block_size, num_blocks,
-                             _stream_ptr(kv_cache.device))
+                             tables.data_ptr(), tables_row, width, lens.data_ptr(), path.data_ptr(), path.shape[1],
+                             counts.data_ptr(), new_lens.data_ptr(), batch, path.shape[1], block_size, num_blocks,
+                             _stream_ptr(device))
     _native.check(rc, "pa_draft_commit")
     return new_lens
