@@ -48,6 +48,9 @@ constexpr int kNodeWords = PA_MAX_DRAFT_NODES / 64;
 constexpr int kBins = 2048;                     // bins of one pass of the search
 constexpr int kVerifyMaxDevices = 64;
 
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+
 struct VerifyParams {
   const void* logits;
   int64_t row_stride, batch_stride;             // elements between nodes, between rows of the batch
@@ -281,84 +284,73 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
   const void* ptr = (const uint8_t*)p.logits + (b * p.batch_stride + node * p.row_stride) * (COUNTS ? 2 : 4);
   const int64_t at = (int64_t)b * p.nodes + node;
   if constexpr (COUNTS) {
-    // The count is bound by the vector ALU: eight instructions for the addresses and increments of a pair of entries.
+    // 2374 atomics a wave and 64 entries for 152k logits, about 8 clocks each at the LDS whatever their addresses: 8 us a row.
+    // In their shadow the largest pattern as a signed number (the maximum, if it is positive) and the smallest as an
+    // unsigned one (the maximum's pattern if all are negative).
     auto add = [&](uint32_t byte, uint32_t inc) __attribute__((always_inline)) {
       __hip_atomic_fetch_add((uint32_t*)__builtin_assume_aligned(lds_raw + byte, 4), inc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    i16x2_t most = {-32768, -32768};
+    u16x2_t least = {65535, 65535};
+    auto note = [&](uint32_t w) __attribute__((always_inline)) {
+      most = __builtin_elementwise_max(most, __builtin_bit_cast(i16x2_t, w));
+      least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2_t, w));
     };
     for_each_logit_pair<DT, kStatThreads, 8>(
         ptr, p.vocab,
         [&](uint32_t w) __attribute__((always_inline)) {
           add((w << 2) & 0x1fffcu, ((w & 0x8000u) << 1) | 1u);
           add((w >> 14) & 0x1fffcu, ((w >> 15) & 0x10000u) | 1u);
+          note(w);
         },
-        [&](uint32_t h) __attribute__((always_inline)) { add((h << 2) & 0x1fffcu, ((h & 0x8000u) << 1) | 1u); },
+        [&](uint32_t h) __attribute__((always_inline)) {
+          add((h << 2) & 0x1fffcu, ((h & 0x8000u) << 1) | 1u);
+          note(h | h << 16);
+        },
         [&]() __attribute__((always_inline)) {       // while the first pieces are on their way
           for (int i = tid; i < WORDS / 4; i += kStatThreads) ((uint4*)hist)[i] = make_uint4(0, 0, 0, 0);
           __syncthreads();
         });
-    __syncthreads();
-    // A wave takes blocks of 512 neighbouring m (wave, 16 + wave, ...), 8 consecutive ones a lane.
-    // Most blocks are empty and cost a read and a test.
-    constexpr int BLOCKS = WORDS / 512, MINE = BLOCKS / kStatWaves;
-    bool seen[MINE];
-    auto words = [&](int m0, uint32_t (&v)[8]) __attribute__((always_inline)) {
-      const uint4 x = ((const uint4*)hist)[m0 / 4], y = ((const uint4*)hist)[m0 / 4 + 1];
-      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-      v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
-    };
-    // entries of +m and of -m that weigh anything
-    auto weighing = [&](uint32_t word, int m, uint32_t& plus, uint32_t& minus) __attribute__((always_inline)) {
-      minus = word >> 16;
-      plus = (word & 0xffffu) - minus;
-      if (m == 0) { plus += minus; minus = 0; }            // -0 and +0 are one value
-      if (m >= INF) minus = 0;                             // -inf
-      if (m > INF) plus = 0;                               // NaN
-    };
-    // the largest value, and the number of entries counted
-    uint32_t pos = 0, neg = 0xffffffffu, count = 0;        // largest m with +m (plus 1), smallest m with -m
-#pragma unroll
-    for (int k = 0; k < MINE; ++k) {
-      uint32_t v[8], any = 0;
-      const int m0 = (wave + kStatWaves * k) * 512 + lane * 8;
-      words(m0, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) any |= v[j];
-      seen[k] = __builtin_amdgcn_ballot_w64(any != 0) != 0;
-      if (!seen[k]) continue;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint32_t plus, minus;
-        weighing(v[j], m0 + j, plus, minus);
-        count += v[j] & 0xffffu;
-        if (plus) pos = m0 + j + 1;
-        if (minus) neg = min(neg, (uint32_t)(m0 + j));
-      }
-    }
+    int high = max(most[0], most[1]);
+    uint32_t low = min(least[0], least[1]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      pos = max(pos, (uint32_t)__shfl_xor(pos, o));
-      neg = min(neg, (uint32_t)__shfl_xor(neg, o));
-      count += __shfl_xor(count, o);
+      high = max(high, __shfl_xor(high, o));
+      low = min(low, (uint32_t)__shfl_xor(low, o));
     }
-    if (lane == 0) { s.redu[0][wave] = pos; s.redu[1][wave] = neg; s.redu[2][wave] = count; }
+    if (lane == 0) { s.redu[0][wave] = (uint32_t)high; s.redu[1][wave] = low; }
     __syncthreads();
-    pos = 0; neg = 0xffffffffu; count = 0;
 #pragma unroll
     for (int w = 0; w < kStatWaves; ++w) {
-      pos = max(pos, s.redu[0][w]);
-      neg = min(neg, s.redu[1][w]);
-      count += s.redu[2][w];
+      high = max(high, (int)s.redu[0][w]);
+      low = min(low, s.redu[1][w]);
     }
-    // a counter that wrapped shows in the total; rows whose maximum is infinite are searched too
-    const bool counted = count == (uint32_t)p.vocab && pos != INF + 1;
-    if (counted && pos == 0 && neg == 0xffffffffu) {       // nothing weighs anything
+    if (high < 0 && low == 0x8000u) high = 0;                // -0 and +0 are one value
+    if (high < 0 && low >= 0x8000u + INF) {                  // all -inf or NaN of that sign: nothing weighs anything
       if (tid == 0) { p.z[at] = 0.0; p.top[at] = p.cut[at] = -INFINITY; }
       return;
     }
-    if (counted) {
+    // A positive NaN hides the maximum, an infinite one makes every other weight 0: both are left to the search.
+    if (high < INF) {
+      // A wave takes blocks of 512 neighbouring m (wave, 16 + wave, ...), 8 consecutive ones a lane.  Most blocks are empty
+      // and cost a read and a test.
+      constexpr int BLOCKS = WORDS / 512, MINE = BLOCKS / kStatWaves;
+      auto words = [&](int m0, uint32_t (&v)[8]) __attribute__((always_inline)) {
+        const uint4 x = ((const uint4*)hist)[m0 / 4], y = ((const uint4*)hist)[m0 / 4 + 1];
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+      };
+      // entries of +m and of -m that weigh anything
+      auto weighing = [&](uint32_t word, int m, uint32_t& plus, uint32_t& minus) __attribute__((always_inline)) {
+        minus = word >> 16;
+        plus = (word & 0xffffu) - minus;
+        if (m == 0) { plus += minus; minus = 0; }            // -0 and +0 are one value
+        if (m >= INF) minus = 0;                             // -inf
+        if (m > INF) plus = 0;                               // NaN
+      };
       auto value = [](int m) { return logit_value<DT>(m); };
-      const float top = pos ? value(pos - 1) : -value(neg);
-      const int top_up = (int)pos - 1, top_down = pos ? 0 : (int)neg;
+      const int top_up = high, top_down = high >= 0 ? 0 : (int)(low & 0x7fffu);        // top_up -1 or less: no positive value
+      const float top = high >= 0 ? value(high) : -value(top_down);
       // Masses of a lane's 8 values of one sign, largest value first.  They are evenly spaced (a binade has 128 values or
       // more), so their weights are a geometric sequence from that of the largest one not above the maximum.
       auto masses_up = [&](int m0, double (&mass)[8]) __attribute__((always_inline)) {
@@ -391,65 +383,97 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const Ver
       };
       auto sum8 = [](const double (&x)[8]) { return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])); };
       // block g's mass of positive values to seg[63 - g], of negative ones to seg[64 + g]: descending order of the values
+      uint32_t count = 0;
 #pragma unroll
       for (int k = 0; k < MINE; ++k) {
         const int g = wave + kStatWaves * k, m0 = g * 512 + lane * 8;
         double up = 0.0, down = 0.0;
-        if (seen[k]) {
-          double mass[8];
-          masses_up(m0, mass);
-          up = wave_scan(sum8(mass));
-          masses_down(m0, mass);
-          down = wave_scan(sum8(mass));
+        uint32_t v[8], any = 0;
+        words(m0, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          any |= v[j];
+          count += v[j] & 0xffffu;
+        }
+        if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
+          if (g > 0 && g < INF / 512 && top_down <= g * 512 && (top_up < g * 512 || top_up >= g * 512 + 511)) {
+            // neither zero nor infinity nor the maximum inside: the polynomials in `fall`, nothing to leave out
+            const double fall = exp2_down(-(double)(value(m0 + 1) - value(m0)) * p.c);
+            double a = 0.0, d = 0.0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a = fma(a, fall, (double)((v[j] & 0xffffu) - (v[j] >> 16)));
+#pragma unroll
+            for (int j = 7; j >= 0; --j) d = fma(d, fall, (double)(v[j] >> 16));
+            // above the maximum there is nothing to weigh
+            up = top_up < g * 512 ? 0.0 : a * exp2_down(((double)value(m0 + 7) - (double)top) * p.c);
+            down = d * exp2_down((-(double)value(m0) - (double)top) * p.c);
+          } else {
+            double mass[8];
+            masses_up(m0, mass);
+            up = sum8(mass);
+            masses_down(m0, mass);
+            down = sum8(mass);
+          }
+          up = wave_scan(up);
+          down = wave_scan(down);
         }
         if (lane == 63) { s.seg[BLOCKS - 1 - g] = up; s.seg[BLOCKS + g] = down; }
       }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) count += __shfl_xor(count, o);
+      if (lane == 0) s.redu[2][wave] = count;
       __syncthreads();
-      // every wave: the block past which the mass exceeds top_p of all
-      const double first = s.seg[2 * lane], second = s.seg[2 * lane + 1];
-      const double upto = wave_scan(first + second);
-      const double z = wave_at(upto, 63), limit = p.top_p * z;
-      const unsigned long long past = p.top_p < 1.0 ? __builtin_amdgcn_ballot_w64(upto > limit) : 0;
-      if (!past) {                                         // everything stays
-        if (tid == 0) { p.z[at] = z; p.top[at] = top; p.cut[at] = -INFINITY; }
+      count = 0;
+#pragma unroll
+      for (int w = 0; w < kStatWaves; ++w) count += s.redu[2][w];
+      // a counter that wrapped shows in the total
+      if (count == (uint32_t)p.vocab) {
+        // every wave: the block past which the mass exceeds top_p of all
+        const double first = s.seg[2 * lane], second = s.seg[2 * lane + 1];
+        const double upto = wave_scan(first + second);
+        const double z = wave_at(upto, 63), limit = p.top_p * z;
+        const unsigned long long past = p.top_p < 1.0 ? __builtin_amdgcn_ballot_w64(upto > limit) : 0;
+        if (!past) {                                         // everything stays
+          if (tid == 0) { p.z[at] = z; p.top[at] = top; p.cut[at] = -INFINITY; }
+          return;
+        }
+        const int l = __builtin_ctzll(past);
+        double above = wave_at(upto, l) - wave_at(first, l) - wave_at(second, l);
+        int o = 2 * l;
+        if (above + wave_at(first, l) <= limit) { above += wave_at(first, l); ++o; }
+        const bool positive = o < BLOCKS;
+        const int g = positive ? BLOCKS - 1 - o : o - BLOCKS;
+        if (g % kStatWaves != wave) return;
+        // the wave that holds the block: its masses in descending order, lanes from 63 down for positive values
+        double mass[8];
+        const int m0 = g * 512 + lane * 8;
+        if (positive) masses_up(m0, mass);
+        else masses_down(m0, mass);
+        const double own = sum8(mass), scan = wave_scan(own);
+        double run = above + (positive ? wave_at(scan, 63) - scan : scan - own);       // mass above this lane's values
+        int cross = 8, some = -1;
+        double kept = 0.0, kept_some = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          run += mass[j];
+          if (mass[j] > 0.0) {
+            some = j;
+            kept_some = run;
+            if (cross == 8 && run > limit) { cross = j; kept = run; }
+          }
+        }
+        const unsigned long long hit = __builtin_amdgcn_ballot_w64(cross < 8), any = __builtin_amdgcn_ballot_w64(some >= 0);
+        // the first value past the limit; where rounding leaves none, the block's last
+        const int who = hit ? (positive ? 63 - __builtin_clzll(hit) : __builtin_ctzll(hit))
+                            : (positive ? __builtin_ctzll(any | 1ull << 63) : 63 - __builtin_clzll(any | 1ull));
+        if (lane == who) {
+          const int j = hit ? cross : max(some, 0);
+          p.z[at] = hit ? kept : some >= 0 ? kept_some : run;
+          p.top[at] = top;
+          p.cut[at] = positive ? value(m0 + 7 - j) : -value(m0 + j);
+        }
         return;
       }
-      const int l = __builtin_ctzll(past);
-      double above = wave_at(upto, l) - wave_at(first, l) - wave_at(second, l);
-      int o = 2 * l;
-      if (above + wave_at(first, l) <= limit) { above += wave_at(first, l); ++o; }
-      const bool positive = o < BLOCKS;
-      const int g = positive ? BLOCKS - 1 - o : o - BLOCKS;
-      if (g % kStatWaves != wave) return;
-      // the wave that holds the block: its masses in descending order, lanes from 63 down for positive values
-      double mass[8];
-      const int m0 = g * 512 + lane * 8;
-      if (positive) masses_up(m0, mass);
-      else masses_down(m0, mass);
-      const double own = sum8(mass), scan = wave_scan(own);
-      double run = above + (positive ? wave_at(scan, 63) - scan : scan - own);       // mass above this lane's values
-      int cross = 8, some = -1;
-      double kept = 0.0, kept_some = 0.0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        run += mass[j];
-        if (mass[j] > 0.0) {
-          some = j;
-          kept_some = run;
-          if (cross == 8 && run > limit) { cross = j; kept = run; }
-        }
-      }
-      const unsigned long long hit = __builtin_amdgcn_ballot_w64(cross < 8), any = __builtin_amdgcn_ballot_w64(some >= 0);
-      // the first value past the limit; where rounding leaves none, the block's last
-      const int who = hit ? (positive ? 63 - __builtin_clzll(hit) : __builtin_ctzll(hit))
-                          : (positive ? __builtin_ctzll(any | 1ull << 63) : 63 - __builtin_clzll(any | 1ull));
-      if (lane == who) {
-        const int j = hit ? cross : max(some, 0);
-        p.z[at] = hit ? kept : some >= 0 ? kept_some : run;
-        p.top[at] = top;
-        p.cut[at] = positive ? value(m0 + 7 - j) : -value(m0 + j);
-      }
-      return;
     }
   }
   __syncthreads();
