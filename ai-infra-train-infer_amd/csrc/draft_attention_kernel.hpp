@@ -82,6 +82,11 @@ __device__ __forceinline__ int draft_keys(const DraftParams& p, int b) {
 // Work unit u of a partitioned launch -> (row, partition), the partitions that hold tokens first: the numbering of
 // unit_to_row_partition, whole partitions before the rows' last ones.
 __device__ __forceinline__ bool draft_unit(const DraftParams& p, int u, int lane, int& row, int& part) {
+  if (p.batch == 1) {                // nothing to look for: a lone sequence is waited for
+    row = 0;
+    part = u;
+    return u * (int64_t)p.partition_size < draft_keys(p, 0);
+  }
   const int per_lane = (p.batch + 63) >> 6;
   const int first = lane * per_lane;
   auto whole_of = [&](int r) { return min(draft_keys(p, r) / p.partition_size, p.max_partitions); };
@@ -147,31 +152,34 @@ __device__ __forceinline__ bool draft_tame(mword4_t& v) {
   return wild;
 }
 
+template <class T>
+using lds_ptr = __attribute__((address_space(3))) T*;
+__device__ __forceinline__ uint32_t lds_offset(const uint8_t* p) { return (uint32_t)(uintptr_t)(lds_ptr<const uint8_t>)p; }
+
 // LDS bytes of a 32-token tile of K, or of V
 __host__ __device__ constexpr int draft_half_bytes(int D) { return kMfmaTile * D * 2; }
 
 // What a wave keeps of its 16 C rows, and one step of them over 32 tokens in LDS.  Result layout of the products: lane
 // (col, kg) holds, for row 16 c + col, keys 4 kg .. + 3 of a 16-key half (scores) or dims 16 mt + 4 kg .. + 3 (output).
-// AHEAD: a step asks for V's fragments before its softmax (32 registers more at head_dim 128).
-template <int KV, int CT, int D, int C, bool AHEAD = true>
+// AHEAD: a step asks for V's fragments before its softmax (32 registers at head_dim 128): for the wide workgroups, which have
+// them; with 16 rows it makes no difference (184 us for 64 rows of 5 nodes x 4096 tokens either way), with 32 they do not fit.
+template <int KV, int CT, int D, int C, bool AHEAD>
 struct DraftRows {
   static constexpr int KSTEPS = D / 32, MT = D / 16, ROWB = D * 2, CPR = D / 8;
   mword4_t q[C][KSTEPS];         // Q^T as the B operand: dims 32 s + 8 kg .. + 7 of row 16 c + col
   mfloat4_t o[C][MT];
   float m_ref[C];                // reference maximum in log2 units, the same in a row's 4 lanes; -inf: nothing seen
   float l_run[C];                // this lane's share of the row's sum
-  uint32_t k_off[KSTEPS], v_off[MT];
+  uint32_t k_first, v_first;     // this lane's K fragment of dims 0 .. 31 and V fragment of dims 0 .. 15 in a tile
   int col, kg;
 
   __device__ __forceinline__ void init(int lane) {
     col = lane & 15;
     kg = lane >> 4;
-#pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) k_off[s] = col * ROWB + (((4 * s + kg) ^ lds_swz<CPR>(col)) << 4);
+    k_first = col * ROWB + ((kg ^ lds_swz<CPR>(col)) << 4);
     // V^T through the transpose read: within a block of 16 lanes lane a supplies the address of 4 dims of key 4 kg + a / 4
     const int key = 4 * kg + (col >> 2);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) v_off[mt] = key * ROWB + (((2 * mt + ((col & 3) >> 1)) ^ lds_swz<CPR>(key)) << 4) + (col & 1) * 8;
+    v_first = key * ROWB + ((((col & 3) >> 1) ^ lds_swz<CPR>(key)) << 4) + (col & 1) * 8;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       m_ref[c] = -INFINITY;
@@ -203,6 +211,21 @@ struct DraftRows {
     else load(std::integral_constant<int, PA_DTYPE_F32>{});
   }
 
+  // Fragments of a 32-token tile at `tile` (of 256 bytes' alignment: a 16-byte piece's number is exclusive-ored with the row's
+  // swizzle, and so may the fragment's number be with the address).  K's fragment i: dims
+  // 32 (i / 2) + 8 kg .. + 7 of key 16 (i % 2) + col.
+  __device__ __forceinline__ mword4_t load_k(uint32_t tile, int i) const {
+    return *(lds_ptr<mword4_t>)(((tile + k_first) ^ (uint32_t)(i >> 1 << 6)) + (i & 1) * 16 * ROWB);
+  }
+  // V^T's: dims 16 mt + col of keys 4 kg .. + 3 and 16 + 4 kg .. + 3
+  __device__ __forceinline__ mword4_t load_v(uint32_t tile, int mt) const {
+    const uint32_t at = (tile + v_first) ^ (uint32_t)(mt << 5);
+    const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_ptr<mfp16x4_t>)at);
+    const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_ptr<mfp16x4_t>)(at + 16 * ROWB));
+    const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+    return mword4_t{l2.x, l2.y, h2.x, h2.y};
+  }
+
   // k, v: the tile in LDS; iks, mvs: per token 1 / k_scale and the mantissa of 1 / v_scale (fp8).  visible(c): bit k =
   // the row sees key k, asked for only in special tiles.
   template <class Visible>
@@ -215,29 +238,18 @@ struct DraftRows {
       for (int kb = 0; kb < 2; ++kb) s[c][kb] = mfloat4_t{0.0f, 0.0f, 0.0f, 0.0f};
     // All of K's fragments are requested before the first product, all of V's before the softmax: left to the scheduler a
     // product waits for the read issued just before it.
-    mword4_t ka[KSTEPS][2];
+    mword4_t f[MT];
+    const uint32_t k_at = lds_offset(k), v_at = lds_offset(v);
 #pragma unroll
-    for (int st = 0; st < KSTEPS; ++st)
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) ka[st][kb] = *(const mword4_t*)(k + k_off[st] + kb * 16 * ROWB);
+    for (int i = 0; i < MT; ++i) f[i] = load_k(k_at, i);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int st = 0; st < KSTEPS; ++st)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int c = 0; c < C; ++c) s[c][kb] = draft_mfma<CT>(ka[st][kb], q[c][st], s[c][kb]);
-    auto load_v = [&](int mt) __attribute__((always_inline)) {
-      const uint8_t* at = v + v_off[mt];
-      const mfp16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)at);
-      const mfp16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) mfp16x4_t*)(at + 16 * ROWB));
-      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-      return mword4_t{l2.x, l2.y, h2.x, h2.y};
-    };
-    mword4_t va[AHEAD ? MT : 1];
+      for (int c = 0; c < C; ++c) s[c][i & 1] = draft_mfma<CT>(f[i], q[c][i >> 1], s[c][i & 1]);
     if constexpr (AHEAD) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) va[mt] = load_v(mt);
+      for (int mt = 0; mt < MT; ++mt) f[mt] = load_v(v_at, mt);
       __builtin_amdgcn_sched_barrier(0);
     }
     mfloat4_t mvs[2];
@@ -310,7 +322,7 @@ struct DraftRows {
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const mword4_t a = AHEAD ? va[AHEAD ? mt : 0] : load_v(mt);
+      const mword4_t a = AHEAD ? f[mt] : load_v(v_at, mt);
 #pragma unroll
       for (int c = 0; c < C; ++c) o[c][mt] = draft_mfma<CT>(a, pb[c], o[c][mt]);
     }
@@ -485,13 +497,13 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
   constexpr bool LM = kLaneMajorTokens<KV>;
   constexpr int WAVEB = decode_mfma_wave_bytes(1, D);
 
-  extern __shared__ __align__(16) uint8_t lds_raw[];
+  extern __shared__ __align__(256) uint8_t draft_lds[];       // fragments' addresses want it (DraftRows)
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  uint8_t* my_lds = lds_raw + wave * WAVEB;
+  uint8_t* my_lds = draft_lds + wave * WAVEB;
   float* my_scales = reinterpret_cast<float*>(my_lds + 2 * draft_half_bytes(D));
-  float (*red)[NC * D] = reinterpret_cast<float (*)[NC * D]>(lds_raw);             // [W][16 x D], over the tiles, one operand at a time
-  float (*sm)[W] = reinterpret_cast<float (*)[W]>(lds_raw + W * WAVEB);            // [16 C][W]
+  float (*red)[NC * D] = reinterpret_cast<float (*)[NC * D]>(draft_lds);             // [W][16 x D], over the tiles, one operand at a time
+  float (*sm)[W] = reinterpret_cast<float (*)[W]>(draft_lds + W * WAVEB);            // [16 C][W]
   float (*sl)[W] = sm + C * NC;
   int* any_wild = reinterpret_cast<int*>(sl + C * NC);         // a drafted token's V holds infinities or NaN
 
@@ -501,14 +513,9 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
   const bool some = draft_work<C * NC, D>(p, w);
   draft_zero_dead<W * 64, D>(p, w);
   if (!some) return;
-  DraftRows<KV, CT, D, C, C == 1> rows;       // with two operands V's fragments ahead of time would not fit 256 registers
+  DraftRows<KV, CT, D, C, false> rows;
   rows.init(lane);
   const int col = rows.col, kg = rows.kg;
-  // rows without a node repeat the last one; they are never written
-  rows.load_q(p.q, p.q_dtype, [&](int c) {
-    const int r = w.row0 + min(16 * c + col, w.live - 1);
-    return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
-  });
 
   if (threadIdx.x == 0) *any_wild = 0;
   __syncthreads();
@@ -621,12 +628,17 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
       int ids[4], ids_next[4];
       load_ids(wave, ids);
       issue_as(stream_tag, t, wave, ids);
-      if (n_mine > 1) load_ids(wave + W, ids);
+      // The queries while the first tile is on its way.  Rows without a node repeat the last one; they are never written.
+      rows.load_q(p.q, p.q_dtype, [&](int c) {
+        const int r = w.row0 + min(16 * c + col, w.live - 1);
+        return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
+      });
+      load_ids(wave + W, ids);
       for (int i = 0; i < n_mine; ++i) {
         const int tile = wave + i * W;
         const int first = begin + tile * TILE;
         const bool special = first + TILE > w.ctx || first + TILE > end;     // drafted tokens or the end inside
-        if (i + 2 < n_mine) load_ids(tile + 2 * W, ids_next);
+        load_ids(tile + 2 * W, ids_next);
         write_tile(t, tile, special);
         if (i + 1 < n_mine) issue_as(stream_tag, t, tile + W, ids);
         rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, p.scale_log2e, special, [&](int c) { return draft_visible(p, w, 16 * c + col, first); });
@@ -693,7 +705,7 @@ __host__ __device__ constexpr int draft_wide_stage_bytes(int D, int WR) {
 }
 __host__ __device__ constexpr int draft_wide_lds_bytes(int D, int WR) { return draft_wide_stage_bytes(D, WR) + 2 * 2 * kWideTile * 4 + 16; }
 
-template <int KV, int CT, int D, int WR>
+template <int KV, int CT, int D, int WR, bool STREAM>
 __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kernel(const DraftParams p) {
   constexpr int W = draft_wide_waves(WR), NT = W * 64;
   constexpr int TK = kWideTile;
@@ -709,9 +721,9 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
   constexpr int MT = D / 16;
   constexpr int TILEB = TK * ROWB;           // the tile's K or V
 
-  extern __shared__ __align__(16) uint8_t lds_raw[];
+  extern __shared__ __align__(256) uint8_t draft_lds[];       // fragments' addresses want it (DraftRows)
   // stage: K, V; then per stage 1 / k_scale and the mantissa of 1 / v_scale; then any_wild
-  float* scales = reinterpret_cast<float*>(lds_raw + draft_wide_stage_bytes(D, WR));
+  float* scales = reinterpret_cast<float*>(draft_lds + draft_wide_stage_bytes(D, WR));
   int* any_wild = reinterpret_cast<int*>(scales + 2 * 2 * TK);        // a drafted token's V holds infinities or NaN
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -722,13 +734,9 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
   const int wr = wave >> 1, wk = wave & 1;
   const bool active = wr < WR && 32 * wr < w.live;         // the wave has rows (it fetches tiles in any case)
   const int row_w = 32 * wr;
-  DraftRows<KV, CT, D, C> rows;
+  DraftRows<KV, CT, D, C, true> rows;
   rows.init(lane);
   const int col = rows.col, kg = rows.kg;
-  rows.load_q(p.q, p.q_dtype, [&](int c) {
-    const int r = w.row0 + min(row_w + 16 * c + col, w.live - 1);
-    return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
-  });
 
   const int begin = w.begin, end = w.end;
   const int bs_mask = (1 << p.bs_log2) - 1;
@@ -740,8 +748,6 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
   const int lrow = tid / LPR;                // this thread's row of a load instruction
   const bool fetches = LPR * TK >= NT || lrow < TK;      // narrow fp8 rows need only part of the workgroup
   const uint32_t lane_off = (uint32_t)(w.kvh * D * ES + (tid % LPR) * 16);
-  // non-temporal loads where nobody else reads the range: no second row tile, no neighbour with the same blocks
-  const bool stream = p.row_tiles == 1 && decode_range_is_private(bt_row, p.bt_stride, w.b, p.batch, min(begin >> p.bs_log2, last_blk));
 
   struct Stage {                             // a tile as loaded
     mword4_t k[NIT], v[NIT];
@@ -754,39 +760,39 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
     for (int i = 0; i < NIT; ++i) ids[i] = bt_row[min((begin + tile * TK + i * RPI + lrow) >> p.bs_log2, last_blk)];
   };
   // The next tile's table entries are asked for before this tile's data: loads return in order, and a wait for entries asked
-  // for behind the data would be a wait for the data.
+  // for behind the data would be a wait for the data.  Past the last tile everybody loads the pool's first token: a wait is for
+  // a number of loads, so loads under a condition would make it one for all of them.
   auto issue = [&](Stage& t, int tile) __attribute__((always_inline)) {
     int now[NIT];
 #pragma unroll
     for (int i = 0; i < NIT; ++i) now[i] = ids[i];
     load_ids(tile + 1);
-    if (tile < ntiles && fetches) {
+    const bool real = tile < ntiles && fetches;
 #pragma unroll
-      for (int i = 0; i < NIT; ++i) {
-        const uint32_t phys = (uint32_t)min(max(now[i], 0), p.num_blocks - 1);
-        const uint32_t off = (uint32_t)((begin + tile * TK + i * RPI + lrow) & bs_mask);
-        const uint64_t base = (uint64_t)phys * block_bytes + off * token_bytes + lane_off;
-        const mword4_t* kp = (const mword4_t*)(p.k_cache + base);
-        const mword4_t* vp = (const mword4_t*)(p.v_cache + base);
-        if (stream) {
-          t.k[i] = __builtin_nontemporal_load(kp);
-          t.v[i] = __builtin_nontemporal_load(vp);
-        } else {
-          t.k[i] = *kp;
-          t.v[i] = *vp;
-        }
-        if constexpr (KV == KV_FP8) {
-          const uint64_t slot = ((uint64_t)phys << p.bs_log2) + off;
-          t.ks[i] = p.k_scale[slot];
-          t.vs[i] = p.v_scale[slot];
-        }
+    for (int i = 0; i < NIT; ++i) {
+      const uint32_t phys = real ? (uint32_t)min(max(now[i], 0), p.num_blocks - 1) : 0u;
+      const uint32_t off = real ? (uint32_t)((begin + tile * TK + i * RPI + lrow) & bs_mask) : 0u;
+      const uint64_t base = (uint64_t)phys * block_bytes + off * token_bytes + (real ? lane_off : 0u);
+      const mword4_t* kp = (const mword4_t*)(p.k_cache + base);
+      const mword4_t* vp = (const mword4_t*)(p.v_cache + base);
+      if constexpr (STREAM) {
+        t.k[i] = __builtin_nontemporal_load(kp);
+        t.v[i] = __builtin_nontemporal_load(vp);
+      } else {
+        t.k[i] = *kp;
+        t.v[i] = *vp;
+      }
+      if constexpr (KV == KV_FP8) {
+        const uint64_t slot = ((uint64_t)phys << p.bs_log2) + off;
+        t.ks[i] = p.k_scale[slot];
+        t.vs[i] = p.v_scale[slot];
       }
     }
   };
   auto commit = [&](Stage& t, int tile) __attribute__((always_inline)) {
     if (tile >= ntiles || !fetches) return;
     const int buf = tile & 1;
-    uint8_t* kt = lds_raw + buf * 2 * TILEB;
+    uint8_t* kt = draft_lds + buf * 2 * TILEB;
     const int past = begin + (tile + 1) * TK;
     const bool special = past > w.ctx || past > end;
     bool wild = false;
@@ -824,11 +830,10 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
     if (special && wild) *any_wild = 1;
   };
   auto compute = [&](int tile) __attribute__((always_inline)) {
-    if (!active) return;
-    const uint8_t* kt = lds_raw + (tile & 1) * 2 * TILEB;
-    const float* sc = scales + (tile & 1) * 2 * TK;
     const int at = wk * (TK / 2), first = begin + tile * TK + at;
-    if (first >= end) return;
+    if (!active || first >= end) return;
+    const uint8_t* kt = draft_lds + (tile & 1) * 2 * TILEB;
+    const float* sc = scales + (tile & 1) * 2 * TK;
     const bool special = first + 32 > w.ctx || first + 32 > end;       // drafted tokens or the end inside
     rows.step(kt + at * ROWB, kt + TILEB + at * ROWB, sc + at, sc + TK + at, p.scale_log2e, special,
               [&](int c) { return draft_visible(p, w, row_w + 16 * c + col, first); });
@@ -838,23 +843,26 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
   load_ids(0);
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) issue(st[d], d);
+  // the queries while the first tiles are on their way
+  rows.load_q(p.q, p.q_dtype, [&](int c) {
+    const int r = w.row0 + min(row_w + 16 * c + col, w.live - 1);
+    return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
+  });
   __syncthreads();
   commit(st[0], 0);
   issue(st[0], DEPTH);
   __syncthreads();
-  // before step `tile`: its tile is in LDS, tiles + 1 ... + DEPTH are on their way, tile t in st[t % DEPTH]
+  // before a turn its tile is in LDS and tiles + 1 ... + DEPTH are on their way, tile t in st[t % DEPTH]
+  auto turn = [&](Stage& next, int t) __attribute__((always_inline)) {
+    compute(t);
+    commit(next, t + 1);             // the other stage: its last readers passed the barrier before this tile
+    issue(next, t + 1 + DEPTH);
+    __syncthreads();
+  };
+  // no way out between the turns of a pair: where such paths meet, waits are for the fewest loads that any of them left
   for (int tile = 0; tile < ntiles; tile += DEPTH) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      const int t = tile + d;
-      if (d == 0 || t < ntiles) {
-        compute(t);
-        Stage& next = st[(d + 1) % DEPTH];
-        commit(next, t + 1);         // the other stage: its last readers passed the barrier before this tile
-        issue(next, t + 1 + DEPTH);
-        __syncthreads();
-      }
-    }
+    turn(st[1 % DEPTH], tile);
+    if constexpr (DEPTH == 2) turn(st[0], tile + 1);
   }
 
   // ---- merge the halves, write --------------------------------------------------------------------------------------
@@ -866,7 +874,7 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
     sum[c] += __shfl_xor(sum[c], 32);
     top[c] = rows.m_ref[c];
   }
-  float* other = reinterpret_cast<float*>(lds_raw) + wr * (32 * (D + 4));  // [32][D + 4]: output, maximum, sum
+  float* other = reinterpret_cast<float*>(draft_lds) + wr * (32 * (D + 4));  // [32][D + 4]: output, maximum, sum
   if (active && wk == 1) {
 #pragma unroll
     for (int c = 0; c < C; ++c) {
@@ -923,8 +931,13 @@ int launch_draft_narrow(const DraftParams& p, unsigned grid, hipStream_t st) {
 
 template <int KV, int CT, int D, int WR>
 int launch_draft_wide(const DraftParams& p, unsigned grid, hipStream_t st) {
-  static std::atomic<bool> attr_set[64];
-  return launch_draft_kernel(draft_wide_kernel<KV, CT, D, WR>, draft_wide_waves(WR) * 64, draft_wide_lds_bytes(D, WR), attr_set, p, grid, st);
+  static std::atomic<bool> attr_set[2][64];
+  // Non-temporal loads where no second row tile reads the same range: 104 us instead of 109 for 32 rows of 64 nodes x 4096
+  // tokens, and no loss where all rows share their blocks (98 us either way).  64-row workgroups gain nothing (153 us).
+  if constexpr (WR == 4)
+    if (p.row_tiles == 1)
+      return launch_draft_kernel(draft_wide_kernel<KV, CT, D, WR, true>, draft_wide_waves(WR) * 64, draft_wide_lds_bytes(D, WR), attr_set[1], p, grid, st);
+  return launch_draft_kernel(draft_wide_kernel<KV, CT, D, WR, false>, draft_wide_waves(WR) * 64, draft_wide_lds_bytes(D, WR), attr_set[0], p, grid, st);
 }
 
 template <int KV, int CT, int D>

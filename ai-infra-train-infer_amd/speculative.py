@@ -127,19 +127,20 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
 
 
 # ---- how an attention launch is shaped -----------------------------------------------------------------------
-# Rows (node, query head of a group) a workgroup serves from one pass over K and V -> workgroups a CU holds at once, what
-# a launch of them costs at least and what one needs per token (ns).  A launch lasts as long as its rounds of workgroups,
-# plus what the memory system needs for all of them together (bytes from HBM once, from the L2 once per row tile; what fits
-# the L2 is all but free there); a split adds the merge pass and the partial results it writes and reads.  Fitted to a sweep
-# of tiles and splits on an MI355X (batch 1 to 64, 5 to 64 nodes, 512 to 32k tokens, ratios of 2 and 8): within 10 % of the
-# best split of the sweep, 20 % at worst (launches of 20 us).
-_DRAFT_TILES = {16: (2, 5000.0, 8.5), 32: (2, 6000.0, 10.0), 64: (2, 8000.0, 17.0), 128: (1, 9000.0, 19.0)}
-_DRAFT_MERGE_NS = (4500.0, 30.0)     # the pass, per partition
-_DRAFT_HBM_BYTES_PER_NS = 6300.0
-_DRAFT_L2_BYTES_PER_NS = 14000.0
-_DRAFT_L2_HOLDS = 64 << 20
-_DRAFT_PARTIAL_BYTES_PER_NS = 4000.0
-_DRAFT_MIN_PARTITION = 128           # tokens: one 32-token tile for each of a workgroup's 4 waves
+# Rows (node, query head of a group) a workgroup serves from one pass over K and V -> workgroups a CU holds at once, what a
+# token costs (ns) a workgroup that has its CU to itself and one that shares it, what a round of workgroups costs besides (ns),
+# the bytes per ns that a launch of them draws from HBM.  A launch lasts as long as its rounds of workgroups and the memory
+# need, neither quite hidden behind the other; a split adds the merge pass and the partial results it writes and reads.
+# Fitted to a sweep of tiles and splits on an MI355X (19 shapes: batch 1 to 64, 5 to 64 nodes, 512 to 32k tokens, ratios of 2
+# to 8, head_dim 128, fp16, bf16 and fp8 caches): the choice is within 2 % of the sweep's best on average, 9 % at worst.  Wide
+# workgroups pay also where they are half empty, since they have the most loads in flight: 24 rows of 10 nodes x 4 query heads
+# a KV head x 3000 tokens take 58 us with 128 rows a workgroup, 69 with 64, 95 with 32.
+_DRAFT_TILES = {16: (2, 9.4, 8.4, 3000.0, 6000.0), 32: (2, 9.8, 8.6, 5900.0, 6600.0), 64: (2, 18.0, 11.3, 3100.0, 7100.0),
+                128: (1, 16.6, 16.6, 5100.0, 9000.0)}
+_DRAFT_LAUNCH_NS = 5000.0
+_DRAFT_MERGE_NS = (2200.0, 3.0)      # the pass, per partition
+_DRAFT_PARTIAL_BYTES_PER_NS = 2550.0
+_DRAFT_MIN_PARTITION = 96            # tokens
 _DRAFT_MAX_PARTITIONS = 64
 
 
@@ -151,21 +152,19 @@ def _choose_draft_launch(batch, nodes, num_q_heads, num_kv_heads, head_dim, elem
     # a batch of unequal rows: a row of the mean length counts its whole partitions and half a one at its end
     ragged = mean_keys < 0.9 * max_keys
     best = None
-    for tile, (per_cu, fixed, token_ns) in _DRAFT_TILES.items():
-        row_tiles = -(-rows // tile)
-        if tile > 16 and 2 * rows <= tile:
+    for tile, (per_cu, alone, shared, round_ns, rate) in _DRAFT_TILES.items():
+        if tile > 16 and 4 * rows <= tile:
             continue
-        memory = read / _DRAFT_HBM_BYTES_PER_NS
-        if read > _DRAFT_L2_HOLDS:
-            memory = max(memory, read * row_tiles / _DRAFT_L2_BYTES_PER_NS)
+        row_tiles = -(-rows // tile)
+        memory = read / rate
+        full = max(alone, per_cu * shared) if per_cu > 1 else alone
         for want in range(1, min(_DRAFT_MAX_PARTITIONS, -(-max_keys // _DRAFT_MIN_PARTITION)) + 1):
             size = -(-(-(-max_keys // want)) // 32) * 32
             parts = -(-max_keys // size)
-            live = batch * (mean_keys / size + 0.5) if ragged else batch * parts
-            rounds = -(-live * num_kv_heads * row_tiles // (per_cu * compute_units))
-            compute = rounds * min(size, max_keys) * token_ns
-            # the 128-row workgroups keep two tiles of loads in flight while they multiply, the others one
-            cost = fixed + (max(memory, compute) + 0.15 * min(memory, compute) if tile == 128 else memory + compute)
+            live = batch * (mean_keys / size + 0.5) if ragged and parts > 1 else batch * parts
+            rounds, rest = divmod(-(-live * num_kv_heads * row_tiles // compute_units), per_cu)
+            compute = min(size, max_keys) * (rounds * full + (alone if rest else 0.0)) + round_ns * (rounds + (1 if rest else 0))
+            cost = _DRAFT_LAUNCH_NS + (memory * memory + compute * compute) ** 0.5
             if parts > 1:
                 partials = live * nodes * num_q_heads * head_dim * 4.0
                 cost += _DRAFT_MERGE_NS[0] + _DRAFT_MERGE_NS[1] * parts + 2.0 * partials / _DRAFT_PARTIAL_BYTES_PER_NS

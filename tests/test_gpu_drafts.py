@@ -545,3 +545,48 @@ def test_commit_refusals(pa, gpu):
         with pytest.raises(RuntimeError, match=text):
             ok(**kw)
     assert pa.commit_drafts(kv, t[:0], lens[:0], path[:0], lens[:0]).shape == (0,)
+
+
+# ---------------------------------------------------------------------------------------------- attention at every width
+
+class OneWidth:
+    """The library with every attention launch at one number of rows a workgroup."""
+
+    def __init__(self, lib, rows):
+        self._lib, self._rows = lib, rows
+
+    def __getattr__(self, name):
+        return getattr(self._lib, name)
+
+    def pa_draft_attention(self, *args):
+        return self._lib.pa_draft_attention(*args[:-2], self._rows, args[-1])
+
+
+@pytest.fixture(params=[16, 32, 64, 128])
+def one_width(request, pa, monkeypatch):
+    from ai_infra_train_infer_amd import _native
+    lib = OneWidth(_native.load(), request.param)
+    monkeypatch.setattr(_native, "load", lambda: lib)
+    return request.param
+
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16"), ("fp8", "bf16"), ("bf16", "fp16"), ("fp16", "fp32")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_types_at_every_width(pa, gpu, one_width, cache, q_type, dim):
+    """Few rows in a wide workgroup and many in narrow ones, tiles from none to several, whole and cut."""
+    for nodes, hq in ((1, 2), (5, 4), (33, 8)):
+        check_attention(pa, gpu, 51 + nodes, [0, 1, 63, 64, 65, 200, 321], nodes, hq, 2, dim, 16, cache, q_type, partitions=(None, 0, 32, 160))
+
+
+def test_attention_padding_and_masks_at_every_width(pa, gpu, one_width):
+    test_attention_padded_rows_and_short_trees(pa, gpu)
+    test_attention_masks_that_leave_a_node_nothing(pa, gpu)
+    test_attention_any_mask_is_taken_as_it_is(pa, gpu)
+    test_attention_scores_far_from_zero(pa, gpu)
+    test_attention_corrupt_tables_stay_inside_the_pool(pa, gpu)
+
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16")])
+def test_attention_nan_and_infinity_at_every_width(pa, gpu, one_width, cache, q_type):
+    test_attention_nan_and_infinity_stay_on_their_branch(pa, gpu, cache, q_type, 6)
+    test_attention_nan_and_infinity_stay_on_their_branch(pa, gpu, cache, q_type, 70)
