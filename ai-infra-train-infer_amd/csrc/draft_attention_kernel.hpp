@@ -67,10 +67,10 @@ struct DraftParams {
   float scale_log2e;
 };
 
-// nodes that row b drafts; 0 also for a context that is no length
+// nodes that row b drafts; 0 also for a context that is no length, or so long that the tiles asked for ahead would pass 32 bits
 __device__ __forceinline__ int draft_nodes(const DraftParams& p, int b) {
   const int ctx = p.context_lens[b];
-  if (ctx < 0 || ctx > 0x7fffffff - 2 * PA_MAX_DRAFT_NODES) return 0;
+  if (ctx < 0 || ctx > 0x7fffffff - 8 * PA_MAX_DRAFT_NODES) return 0;
   return p.num_nodes ? min(max(p.num_nodes[b], 0), p.nodes) : p.nodes;
 }
 // tokens of row b: committed and drafted
@@ -474,7 +474,8 @@ __device__ __forceinline__ void draft_wild(const DraftParams& p, const DraftWork
 
 // ---- up to 32 rows: every wave has its own tokens ----------------------------------------------------------------
 
-// C 16-row operands, 1 or 2.  (8 waves a workgroup in launches of fewer workgroups than CUs changed nothing: a lone
+// C 16-row operands, 1 or 2.  64 rows of 5 nodes x 4096 tokens of an fp8 cache: 101 us, 5.4 TB/s; one row of 5 nodes x 2048
+// tokens: 7.4 us, a chain of five dependent loads (length, table, tile, partial result, merge).  (8 waves a workgroup in launches of fewer workgroups than CUs changed nothing: a lone
 // workgroup is bound by what its CU can pull, about 70 GB/s, and more partitions put more CUs to work.)
 constexpr int kDraftWaves = 4;
 
@@ -693,9 +694,14 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
 // 32 WR rows per workgroup.  A 64-token tile of K and V is fetched by the whole workgroup and staged in LDS, double
 // buffered, one barrier a tile; the next DEPTH tiles' loads are in flight in registers meanwhile.  Wave (wr, wk) takes
 // rows 32 wr .. + 31 of the tile's half wk (WR = 1 with 4 waves: waves 2 and 3 only fetch), and the halves are merged at
-// the end.  8 waves for 128 rows: a CU then holds one workgroup with two waves per SIMD, whose products and exponentials
-// overlap, and 64 KiB of loads in flight (4 waves taking all 64 tokens each, one tile ahead: 32 rows of 64 nodes x 4096
-// tokens took 146 us, of which the loads by themselves were 104).
+// the end.  8 waves for 128 rows: a CU then holds one workgroup with two waves per SIMD and 64 KiB of loads in flight (4 waves
+// taking all 64 tokens each, one tile ahead: 32 rows of 64 nodes x 4096 tokens took 146 us; now 104, 5.2 TB/s, which is what
+// the loads by themselves take).
+// Two row tiles per KV head and long contexts are bound by the turn instead: 4 rows of 27 nodes x 64 heads x 16k to 32k tokens
+// take 162 us (540 TFLOP/s of rows that count), of which the launch and two rounds of first loads and last stores are 44,
+// products and exponentials 82, fetching and staging 36.  A turn is 1.2 us: matrix pipe 0.42, vector ALU 0.55, LDS 0.55, hardly
+// overlapped.  Waves half a turn apart, a third stage with the next fragments read ahead of the barrier, and a raised wave
+// priority during the products left it where it is.
 
 constexpr int kWideTile = 64;
 __host__ __device__ constexpr int draft_wide_waves(int WR) { return WR == 4 ? 8 : 4; }

@@ -756,6 +756,8 @@ class ModelRunner:
         if self.model is None:
             raise RuntimeError("run_drafts: the runner has no model of PagedAttention layers")
         num_blocks = self._kv_cache.shape[2] if self._kv_cache is not None else 2 ** 31 // self.block_size - 1
+        if tokens.dim() != 2 or tokens.shape[1] != parents.shape[-1]:
+            raise RuntimeError("run_drafts: tokens %s do not match the %d nodes of parents" % (tuple(tokens.shape), parents.shape[-1]))
         positions, slots, mask = draft_layout(parents, context_lens, block_tables, self.block_size, num_blocks, num_nodes)
         set_context(is_prefill=False, slot_mapping=slots.view(-1), context_lens=context_lens, block_tables=block_tables,
                     longest_context_len=longest_context, mean_context_len=mean_context, tree_mask=mask, num_nodes=num_nodes)

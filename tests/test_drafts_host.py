@@ -180,6 +180,8 @@ def test_attention_launch_policy(pa):
 
 def test_run_drafts_refuses_a_runner_without_a_model(pa):
     runner = pa.ModelRunner(None, pa.ModelRunnerConfig(block_size=16, device="cpu"))
+    with pytest.raises(RuntimeError, match="tokens"):
+        pa.ModelRunner(torch.nn.Identity(), runner.config).run_drafts(torch.zeros(2, 3).long(), torch.zeros(4).int(), torch.zeros(2, 1).int(), torch.zeros(2).int())
     one = torch.zeros(1, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no model"):
         runner.run_drafts(one.long(), one, one, one[0])
