@@ -52,6 +52,7 @@ constexpr int kChunk = 512;                     // vocabulary entries behind one
 constexpr int kNodeWords = PA_MAX_DRAFT_NODES / 64;
 constexpr int kBins = 2048;                     // bins of one pass of the search
 constexpr int kVerifyMaxDevices = 64;
+constexpr int kSumVocab = 16384;                // 16-bit rows up to here are summed entry by entry where top_p keeps all
 
 typedef short i16x2_t __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
@@ -193,12 +194,13 @@ struct RowStats {
   float top, cut;
 };
 
-// Row statistics without the histogram: maximum, then the sum of all weights, then (top_p < 1) the smallest kept
+// Row statistics without the histogram: maximum, the sum of all weights and, where top_p < 1, the smallest kept
 // logit by a search over ordered bit patterns: the range that holds it is cut into 2048 bins, the weights of the
 // range's entries are added up per bin as 64-bit fixed-point numbers (exact, so the order of the atomics does not
-// matter), and the bin in which the mass above crosses top_p * z is the next range.  The first range starts at the
-// smallest weight that can be kept: tokens lighter than (1 - top_p) z / vocab weigh less than 1 - top_p together.
-// A pass costs one read of the row from the L2 and an exponential per entry in range: 3 passes on 32-bit logits.
+// matter), and the bin in which the mass above crosses top_p * z is the next range.  The first range starts below the
+// smallest weight that can be kept: tokens lighter than (1 - top_p) z / vocab weigh less than 1 - top_p together, and
+// z >= 1.  The first of the 3 passes (32-bit logits) adds up z as well; the later ones need an exponential per entry
+// in range only.  Bound by the exponentials, a row to a CU.
 template <int DT>
 __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t* bins, StatLds& s) {
   const int tid = threadIdx.x;
@@ -215,26 +217,32 @@ __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t*
   r.cut = -INFINITY;
   if (best == -INFINITY) { r.z = 0.0; return r; }
   double mine = 0.0;
-  for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) { mine += logit_weight(x, best, p.c); });
-  r.z = group_sum<kStatWaves>(mine, s.red);
-  if (!(p.top_p < 1.0) || best == INFINITY) return r;
-  const double limit = p.top_p * r.z;
+  if (!(p.top_p < 1.0) || best == INFINITY) {
+    for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) { mine += logit_weight(x, best, p.c); });
+    r.z = group_sum<kStatWaves>(mine, s.red);
+    return r;
+  }
   const int log_vocab = 32 - __builtin_clz((uint32_t)p.vocab);
   const double unit = ldexp(1.0, 62 - log_vocab), back = 1.0 / unit;     // a row's weights sum to at most `vocab`
-  const float low = (float)((double)best + log2((1.0 - p.top_p) * r.z / p.vocab * 0.5) / p.c);
+  const float low = (float)((double)best + log2((1.0 - p.top_p) / p.vocab * 0.5) / p.c);
   uint32_t lo = ordered_key32(low < best ? low : best), hi = ordered_key32(r.top);
-  double above = 0.0;
-  for (;;) {
+  double above = 0.0, limit = 0.0;
+  for (bool first = true;; first = false) {
     const uint32_t span = hi - lo;
     const int shift = span < kBins ? 0 : 21 - __builtin_clz(span);       // span >> shift < 2048
     for (int i = tid; i < kBins; i += kStatThreads) bins[i] = 0;
     __syncthreads();
     for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) {
       const uint32_t off = ordered_key32(x + 0.0f) - lo;                   // -0 counts as +0; NaN lies beyond every finite key
-      if (off <= span)
-        __hip_atomic_fetch_add(&bins[off >> shift], (uint64_t)(logit_weight(x, best, p.c) * unit + 0.5), __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_WORKGROUP);
+      if (!first && off > span) return;
+      const double w = logit_weight(x, best, p.c);
+      if (first) mine += w;
+      if (off <= span) __hip_atomic_fetch_add(&bins[off >> shift], (uint64_t)(w * unit + 0.5), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     });
+    if (first) {
+      r.z = group_sum<kStatWaves>(mine, s.red);
+      limit = p.top_p * r.z;
+    }
     __syncthreads();
     // bins from the top: thread t takes bins 2047 - 2t and 2046 - 2t
     const double m0 = (double)bins[kBins - 1 - 2 * tid] * back, m1 = (double)bins[kBins - 2 - 2 * tid] * back;
@@ -275,18 +283,18 @@ __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t*
 // One workgroup per node.  16-bit logits: LDS holds 32768 words, the entries of bit pattern m in the low half of word m, those
 // of -m (the same with the sign bit) counted in the high half and in the low half too; then StatLds.  32-bit logits: the bins of
 // the search, then StatLds.
-template <int DT>
+template <int DT, bool COUNTS>
 __global__ __launch_bounds__(kStatThreads) void draft_row_stats_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t lds_raw[];
   const int node = blockIdx.x, b = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (node >= nodes_of(p, b)) return;
-  constexpr bool COUNTS = DT != PA_DTYPE_F32;
+  static_assert(!COUNTS || DT != PA_DTYPE_F32, "32-bit patterns are too many to count");
   constexpr int WORDS = 32768;
   constexpr int INF = DT == PA_DTYPE_F16 ? 0x7c00 : 0x7f80;
   uint32_t* hist = (uint32_t*)lds_raw;
   StatLds& s = *(StatLds*)(lds_raw + (COUNTS ? WORDS * 4 : kBins * 8));
-  const void* ptr = (const uint8_t*)p.logits + (b * p.batch_stride + node * p.row_stride) * (COUNTS ? 2 : 4);
+  const void* ptr = (const uint8_t*)p.logits + (b * p.batch_stride + node * p.row_stride) * (DT == PA_DTYPE_F32 ? 4 : 2);
   const int64_t at = (int64_t)b * p.nodes + node;
   if constexpr (COUNTS) {
     // 2374 atomics a wave and 64 entries for 152k logits, about 8 clocks each at the LDS whatever their addresses: 8 us a row.
@@ -858,10 +866,13 @@ static int launch_verify(const VerifyParams& p, int64_t batch, bool greedy, hipS
     hipLaunchKernelGGL((draft_walk_kernel<DT, true>), dim3(1, (unsigned)batch), dim3(kWalkThreads), 0, st, p);
     return check_launch("pa_verify_drafts");
   }
-  auto kern = draft_row_stats_kernel<DT>;
-  const size_t lds = (DT == PA_DTYPE_F32 ? (size_t)kBins * 8 : (size_t)32768 * 4) + sizeof(StatLds);
+  // Clearing and reading 128 KiB of counters takes 7 us a row: not for a short row of which only the sum is wanted.
+  const bool counts = DT != PA_DTYPE_F32 && !(p.top_p >= 1.0 && p.vocab <= kSumVocab);
+  auto kern = counts ? draft_row_stats_kernel<DT, DT != PA_DTYPE_F32> : draft_row_stats_kernel<DT, false>;
+  const size_t lds = (counts ? (size_t)32768 * 4 : (size_t)kBins * 8) + sizeof(StatLds);
   // the attribute belongs to the kernel on one device: once per instantiation and device
-  static std::atomic<bool> attr_set[kVerifyMaxDevices];
+  static std::atomic<bool> attr_sets[2][kVerifyMaxDevices];
+  auto& attr_set = attr_sets[counts];
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kVerifyMaxDevices)
     return fail(PA_ERR_LAUNCH, "pa_verify_drafts: cannot tell the current device");

@@ -590,3 +590,17 @@ def test_attention_padding_and_masks_at_every_width(pa, gpu, one_width):
 def test_attention_nan_and_infinity_at_every_width(pa, gpu, one_width, cache, q_type):
     test_attention_nan_and_infinity_stay_on_their_branch(pa, gpu, cache, q_type, 6)
     test_attention_nan_and_infinity_stay_on_their_branch(pa, gpu, cache, q_type, 70)
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("vocab", [16384, 16385])
+@pytest.mark.parametrize("top_p", [1.0, 2.0, 0.95])
+def test_verify_on_both_sides_of_the_counters(pa, gpu, dtype, vocab, top_p):
+    check_verify(pa, gpu, 61, 4, 9, vocab, dtype, 0.8, top_p)
+    check_verify(pa, gpu, 62, 4, 6, vocab, dtype, 1.0, top_p, kind="chain", probs="fp16")
+
+
+def test_verify_short_rows_with_masked_entries_are_summed(pa, gpu):
+    """Infinities, NaN and rows with nothing left, where the counters are not used."""
+    test_verify_rows_with_masked_and_extreme_logits(pa, gpu, "fp16", 1.0, 1.0)
+    test_verify_rows_with_masked_and_extreme_logits(pa, gpu, "bf16", 0.3, 1.0)
