@@ -403,23 +403,25 @@ def test_verify_short_and_padded_rows(pa, gpu):
     check_verify(pa, gpu, 8, 5, 6, 100, "fp32", 1.0, 1.0, kind="chain", probs="fp32", real=[0, 1, 2, 6, 0])
 
 
+def extreme(x):
+    low = torch.finfo(x.dtype).min
+    x[0, :, 1::2] = -float("inf")
+    x[1, :, 5:] = low
+    x[2, :, ::3] = float("nan")
+    x[3] = 0.0                                            # all equal
+    x[3, :, ::2] = -0.0                                   # of both signs
+    x[4] = -x[4].abs() - 3                                # nothing positive
+    x[5, :, 7] = torch.finfo(x.dtype).max                 # one token takes everything
+    x[6] = low
+    x[7] = -float("inf")                                  # nothing at all
+    x[8] = float("nan")
+    x[9, :, :] = -float("inf")
+    x[9, :, 11] = 2.0                                     # a grammar that leaves one token
+
+
 @pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
 @pytest.mark.parametrize("temperature,top_p", [(1.0, 1.0), (0.7, 0.9), (0.0, 1.0)])
 def test_verify_rows_with_masked_and_extreme_logits(pa, gpu, dtype, temperature, top_p):
-    def extreme(x):
-        low = torch.finfo(x.dtype).min
-        x[0, :, 1::2] = -float("inf")
-        x[1, :, 5:] = low
-        x[2, :, ::3] = float("nan")
-        x[3] = 0.0                                            # all equal
-        x[3, :, ::2] = -0.0                                   # of both signs
-        x[4] = -x[4].abs() - 3                                # nothing positive
-        x[5, :, 7] = torch.finfo(x.dtype).max                 # one token takes everything
-        x[6] = low
-        x[7] = -float("inf")                                  # nothing at all
-        x[8] = float("nan")
-        x[9, :, :] = -float("inf")
-        x[9, :, 11] = 2.0                                     # a grammar that leaves one token
     check_verify(pa, gpu, 13, 10, 5, 200, dtype, temperature, top_p, change=extreme)
 
 
@@ -600,7 +602,7 @@ def test_verify_on_both_sides_of_the_counters(pa, gpu, dtype, vocab, top_p):
     check_verify(pa, gpu, 62, 4, 6, vocab, dtype, 1.0, top_p, kind="chain", probs="fp16")
 
 
-def test_verify_short_rows_with_masked_entries_are_summed(pa, gpu):
-    """Infinities, NaN and rows with nothing left, where the counters are not used."""
-    test_verify_rows_with_masked_and_extreme_logits(pa, gpu, "fp16", 1.0, 1.0)
-    test_verify_rows_with_masked_and_extreme_logits(pa, gpu, "bf16", 0.3, 1.0)
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("top_p", [0.9, 1.0])
+def test_verify_masked_and_extreme_logits_in_counters(pa, gpu, dtype, top_p):
+    check_verify(pa, gpu, 63, 10, 5, 16400, dtype, 1.0, top_p, change=extreme)
