@@ -79,8 +79,20 @@ __device__ __forceinline__ int draft_keys(const DraftParams& p, int b) {
   return n > 0 ? p.context_lens[b] + n : 0;
 }
 
+// Inclusive prefix sum over the lanes of a wave, all of them active: within the rows of 16, then across them.
+__device__ __forceinline__ int draft_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);     // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);     // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
 // Work unit u of a partitioned launch -> (row, partition), the partitions that hold tokens first: the numbering of
-// unit_to_row_partition, whole partitions before the rows' last ones.
+// unit_to_row_partition, whole partitions before the rows' last ones.  Lane l counts those of rows l * per_lane ....  Every
+// workgroup waits for this before its first load.
 __device__ __forceinline__ bool draft_unit(const DraftParams& p, int u, int lane, int& row, int& part) {
   if (p.batch == 1) {                // nothing to look for: a lone sequence is waited for
     row = 0;
@@ -89,21 +101,38 @@ __device__ __forceinline__ bool draft_unit(const DraftParams& p, int u, int lane
   }
   const int per_lane = (p.batch + 63) >> 6;
   const int first = lane * per_lane;
-  auto whole_of = [&](int r) { return min(draft_keys(p, r) / p.partition_size, p.max_partitions); };
-  auto live_of = [&](int r) { return min((draft_keys(p, r) + p.partition_size - 1) / p.partition_size, p.max_partitions); };
+  auto count = [&](int r, int& whole, int& live) __attribute__((always_inline)) {
+    const int keys = draft_keys(p, r), q = keys / p.partition_size;
+    whole = min(q, p.max_partitions);
+    live = min(q + (q * p.partition_size < keys ? 1 : 0), p.max_partitions);
+  };
   int whole = 0, tails = 0;
   for (int i = 0; i < per_lane; ++i)
     if (first + i < p.batch) {
-      const int w = whole_of(first + i);
+      int w, l;
+      count(first + i, w, l);
       whole += w;
-      tails += live_of(first + i) - w;
+      tails += l - w;
     }
-  int total_whole;
-  if (locate_item(whole, u, lane, per_lane, whole_of, row, part, total_whole)) return true;
-  int index, total_tails;
-  if (!locate_item(tails, u - total_whole, lane, per_lane, [&](int r) { return live_of(r) - whole_of(r); }, row, index, total_tails))
-    return false;
-  part = whole_of(row);
+  const int whole_to = draft_scan(whole), tails_to = draft_scan(tails);
+  const int total = __builtin_amdgcn_readlane(whole_to, 63);
+  const bool tail = u >= total;
+  const int want = tail ? u - total : u;
+  const unsigned long long past = __builtin_amdgcn_ballot_w64((tail ? tails_to : whole_to) > want);
+  if (past == 0) return false;
+  const int owner = __builtin_ctzll(past);
+  int base = __builtin_amdgcn_readlane(tail ? tails_to - tails : whole_to - whole, owner), w = __builtin_amdgcn_readlane(whole, owner);
+  row = owner;
+  if (per_lane > 1) {                // the owner's rows hold more than want - base, so the walk ends inside them
+    for (row = owner * per_lane;; ++row) {
+      int l;
+      count(row, w, l);
+      const int c = tail ? l - w : w;
+      if (want < base + c) break;
+      base += c;
+    }
+  }
+  part = tail ? w : want - base;     // a row's last partition comes after its whole ones
   return true;
 }
 

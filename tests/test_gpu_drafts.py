@@ -606,3 +606,13 @@ def test_verify_on_both_sides_of_the_counters(pa, gpu, dtype, vocab, top_p):
 @pytest.mark.parametrize("top_p", [0.9, 1.0])
 def test_verify_masked_and_extreme_logits_in_counters(pa, gpu, dtype, top_p):
     check_verify(pa, gpu, 63, 10, 5, 16400, dtype, 1.0, top_p, change=extreme)
+
+
+@pytest.mark.parametrize("batch", [2, 63, 64, 65, 130])
+def test_attention_many_ragged_rows_in_partitions(pa, gpu, batch):
+    """More rows than lanes, rows of no, one and several partitions, of whole ones only and with a rest."""
+    rng = random.Random(batch)
+    lens = [rng.choice([0, 1, 29, 30, 31, 61, 62, 94, 100, rng.randrange(200)]) for _ in range(batch)]
+    real = [rng.choice([0, 1, 2, 3]) for _ in range(batch)]
+    check_attention(pa, gpu, 71, lens, 3, 2, 1, 64, 16, "fp16", "fp16", real=real, partitions=(32, 64, None))
+    check_attention(pa, gpu, 72, lens, 2, 2, 1, 64, 16, "fp8", "bf16", partitions=(32, 96))
