@@ -32,8 +32,8 @@
 // bits a pass.  Short rows of which top_p keeps all are summed entry by entry.
 //
 // One row of 152k 16-bit logits takes (1) 19.5 us: 8 us of LDS atomics, 5 us to get at the row and clear the counters, 5 us of
-// masses.  64 rows of a chain of 5 with draft probabilities: 22 + 23 + 6 us, 16 rows of a tree of 64: 94 (3.3 TB/s) + 11 + 6 us;
-// 5 rows of 32-bit logits: 107 us the whole call with top_p < 1, 52 without.
+// masses.  64 rows of a chain of 5 with draft probabilities: 22 + 21 + 6 us, 16 rows of a tree of 64: 94 (3.3 TB/s) + 11 + 6 us;
+// 5 rows of 32-bit logits: 97 us the whole call with top_p < 1, 45 without.
 #include "logit_row.hpp"
 #include "pa_common.hpp"
 #include "pa_host.hpp"
@@ -87,7 +87,7 @@ __device__ __forceinline__ int nodes_of(const VerifyParams& p, int b) {
 }
 
 // 2^x for x <= 0 to 2^-51: x = n + f with |f| <= 1/2, the series of e^(f ln 2) to the 12th power (its rest is below
-// (ln 2 / 2)^13 / 13! = 2^-52.2) and the exponent added.  Below 2^-1000: 0.  Half the instructions of the library's exp2, which
+// (ln 2 / 2)^13 / 13! = 2^-52.2) and the exponent added.  0 for NaN and -inf, by the clamp.  Half the instructions of the library's exp2, which
 // also takes every other argument; the row statistics and the sums of the draw are bound by them.
 __device__ __forceinline__ double exp2_down(double x) {
   // (ln 2)^k / k!, held in scalar registers: as literals each costs two moves into the accumulator of its multiply-add
@@ -105,6 +105,7 @@ __device__ __forceinline__ double exp2_down(double x) {
   double c1 = 0.6931471805599453;
   asm("" : "+s"(c12), "+s"(c11), "+s"(c10), "+s"(c9), "+s"(c8), "+s"(c7));
   asm("" : "+s"(c6), "+s"(c5), "+s"(c4), "+s"(c3), "+s"(c2), "+s"(c1));
+  x = fmax(x, -2000.0);
   const double n = __builtin_rint(x), f = x - n;
   double r = fma(c12, f, c11);
   r = fma(r, f, c10);
@@ -118,14 +119,15 @@ __device__ __forceinline__ double exp2_down(double x) {
   r = fma(r, f, c2);
   r = fma(r, f, c1);
   r = fma(r, f, 1.0);
-  return x > -1000.0 ? __builtin_amdgcn_ldexp(r, (int)n) : 0.0;
+  return __builtin_amdgcn_ldexp(r, (int)n);
 }
 
-// w of one logit; NaN and -inf weigh nothing
+// w of one logit of a row with a finite maximum; NaN and -inf weigh nothing
+__device__ __forceinline__ double finite_weight(float l, double top, double c) { return exp2_down(((double)l - top) * c); }
+
+// The same for any maximum: under an infinite one everything else weighs nothing.
 __device__ __forceinline__ double logit_weight(float l, float top, double c) {
-  const double x = l == top ? 0.0 : (double)l - (double)top;
-  const double w = exp2_down(x * c);
-  return l <= top && l > -INFINITY ? w : 0.0;
+  return l == top ? (l > -INFINITY ? 1.0 : 0.0) : finite_weight(l, top, c);
 }
 
 template <int CTRL, int ROWS>
@@ -217,8 +219,13 @@ __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t*
   r.cut = -INFINITY;
   if (best == -INFINITY) { r.z = 0.0; return r; }
   double mine = 0.0;
-  if (!(p.top_p < 1.0) || best == INFINITY) {
-    for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) { mine += logit_weight(x, best, p.c); });
+  if (best == INFINITY) {
+    for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) { mine += x == INFINITY ? 1.0 : 0.0; });
+    r.z = group_sum<kStatWaves>(mine, s.red);
+    return r;
+  }
+  if (!(p.top_p < 1.0)) {
+    for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) { mine += finite_weight(x, best, p.c); });
     r.z = group_sum<kStatWaves>(mine, s.red);
     return r;
   }
@@ -235,7 +242,7 @@ __device__ RowStats search_row(const void* ptr, const VerifyParams& p, uint64_t*
     for_each_logit<DT, kStatThreads>(ptr, p.vocab, [&](int, float x) __attribute__((always_inline)) {
       const uint32_t off = ordered_key32(x + 0.0f) - lo;                   // -0 counts as +0; NaN lies beyond every finite key
       if (!first && off > span) return;
-      const double w = logit_weight(x, best, p.c);
+      const double w = finite_weight(x, best, p.c);
       if (first) mine += w;
       if (off <= span) __hip_atomic_fetch_add(&bins[off >> shift], (uint64_t)(w * unit + 0.5), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
     });
@@ -553,11 +560,18 @@ __device__ __forceinline__ void load_entries(const void* row, int dtype, int i0,
 
 // The weights with which the token after node `last` is drawn, of 8 entries of logits l, and all kept weights.
 // drop: bit e leaves entry e out (a refused child's token).  from_q: drafts drawn from q were refused; inv_z: 1 / z then.
-__device__ __forceinline__ void draw_weights(const VerifyParams& p, const float (&l)[8], const float (&q)[8], bool from_q, float top,
+__device__ __forceinline__ void draw_weights(const VerifyParams& p, float (&l)[8], const float (&q)[8], bool from_q, float top,
                                              float cut, double inv_z, uint32_t drop, double (&drawn)[8], double (&all)[8]) {
+  if (__builtin_expect(top == INFINITY, 0)) {              // such a row keeps all of its infinities
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l[e] = l[e] == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    all[e] = l[e] >= cut ? logit_weight(l[e], top, p.c) : 0.0;
+    all[e] = 0.0;
+    // with top_p few entries are kept, and in most places none of a wave's: 11 us against 12 for 16 rows of 152k
+    if (__builtin_amdgcn_ballot_w64(l[e] >= cut) != 0) all[e] = finite_weight(l[e] >= cut ? l[e] : -INFINITY, top, p.c);
     if (from_q) drawn[e] = fmax(fma(all[e], inv_z, -(double)q[e]), 0.0);
     else drawn[e] = (drop >> e) & 1u ? 0.0 : all[e];
   }
@@ -950,7 +964,8 @@ extern "C" int pa_verify_drafts(const void* logits, int dtype, int64_t row_strid
   p.vocab = (int)vocab;
   p.chunks = (int)((vocab + kChunk - 1) / kChunk);
   // With draft probabilities a wave's chunks are a long chain of loads, exponentials and sums: as many workgroups as the GPU
-  // holds at once, six a CU (64 rows of 152k entries: 27 us with 1536 workgroups, 34 with 512).  Without, the walk that every
+  // holds at once, six a CU (64 rows of 152k entries: 27 us with 1536 workgroups, 34 with 512,
+  // before an exponential lost a third of its instructions; 21 now).  Without, the walk that every
   // workgroup repeats weighs more: half of that (16 rows of 64 nodes: 11 us with 512, 12 with 1024, 14 with 1536).
   const int64_t want = ((p.q ? 1536 : 768) + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
   p.slices = (int)(want < most ? want : most);
