@@ -1,0 +1,84 @@
+"""Speculative decoding on the GPU where values are no ordinary numbers or sizes no ordinary ones: NaN and infinities in
+committed tokens and queries, at every width of a workgroup and split of a row, element by element against the 64-bit oracle."""
+import math
+import random
+
+import pytest
+import torch
+
+from oracle import speculative_oracle as so
+from test_gpu_drafts import DT, FP8, Pool, bound, check_verify, make_parents, one_width      # noqa: F401 (a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def i32(values, gpu):
+    return torch.tensor(values, dtype=torch.int32, device=gpu)
+
+
+def check_elements(pa, gpu, pool, q, lens, sets, partitions, p_type, scale=None, real=None):
+    """Every output element against the oracle: where that is NaN or infinite the output is the same, elsewhere it is within
+    bound().  q [batch, nodes, heads, dim] on the CPU."""
+    batch, nodes, hq, dim = q.shape
+    scale = dim ** -0.5 if scale is None else scale
+    mask = torch.stack([so.mask_words(s, nodes) for s in sets]).to(gpu)
+    k, v, tables, ks, vs = pool.device(gpu)
+    outs = [pa.paged_draft_attention(q.to(gpu), k, v, tables, i32(lens, gpu), mask, scale, ks, vs, partition_size=part,
+                                     num_nodes=None if real is None else i32(real, gpu)).cpu()
+            for part in partitions]
+    odd = 0
+    for b in range(batch):
+        n = nodes if real is None else real[b]
+        kr, vr = (so.row_kv(x, f, pool.tables[b].tolist(), lens[b] + n, pool.block) for x, f in ((pool.k, pool.ks), (pool.v, pool.vs)))
+        want, spread, weight = so.attention(q[b], kr, vr, lens[b], sets[b], n, scale)
+        fine = torch.isfinite(want)
+        odd += int((~fine).sum())
+        for part, out in zip(partitions, outs):
+            got = out[b].double()
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (b, part)
+            assert torch.equal(torch.where(torch.isinf(got), got, 0.0), torch.where(torch.isinf(want), want, 0.0)), (b, part)
+            far, may = (got - want).abs()[fine], bound(want, spread, weight, p_type, q.dtype)[fine]
+            assert (far <= may).all(), (b, part, float((far / may).max()))
+    return odd
+
+
+def poison(t, scales, tables, block, row, pos, head, dims, value):
+    """Token `pos` of a row, one KV head and some dims: NaN or an infinity (fp8: NaN, which is all it has)."""
+    at = (int(tables[row, pos // block]), pos % block, head)
+    if t.dtype == FP8:
+        t.view(torch.uint8)[at][dims] = 0x7F
+    else:
+        t[at][dims] = value
+
+
+TYPES = [("fp16", "fp16"), ("bf16", "bf16"), ("fp8", "fp16"), ("fp16", "bf16"), ("fp8", "fp32")]
+
+
+def product_type(cache, q_type):
+    return torch.bfloat16 if cache == "bf16" and q_type == "bf16" else torch.float16
+
+
+def random_case(seed, lens, nodes, hq, hkv, dim, block, cache, q_type):
+    rng = random.Random(seed)
+    pool = Pool(seed, lens, [nodes] * len(lens), hkv, dim, block, cache)
+    sets = [so.ancestors(make_parents("tree", nodes, rng)) for _ in lens]
+    q = torch.randn(len(lens), nodes, hq, dim, generator=torch.Generator().manual_seed(seed + 1)).to(torch.float16).to(DT[q_type])
+    return pool, sets, q
+
+
+# ---------------------------------------------------------------------------------------------- infinities and NaN
+
+@pytest.mark.parametrize("cache,q_type", TYPES)
+@pytest.mark.parametrize("nodes", [3, 21])
+def test_nan_and_infinity_in_committed_values(pa, gpu, one_width, cache, q_type, nodes):
+    """V of committed tokens anywhere in a split: in its middle, in the last 32 tokens of partitions of an odd multiple of 32,
+    just before the drafted tokens."""
+    lens = [330, 70, 200]
+    pool, sets, q = random_case(3, lens, nodes, 4, 2, 64, 16, cache, q_type)
+    inf, nan = float("inf"), float("nan")
+    for row, pos, head, dims, value in ((0, 70, 0, slice(0, 3), nan), (0, 95, 0, slice(3, 6), inf), (0, 159, 1, slice(8, 9), -inf),
+                                        (0, 130, 1, slice(8, 11), inf), (0, 329, 0, slice(12, 13), inf), (0, 4, 1, slice(63, 64), nan),
+                                        (1, 31, 0, slice(5, 6), -inf), (1, 69, 1, slice(0, 64), nan)):
+        poison(pool.v, pool.vs, pool.tables, 16, row, pos, head, dims, value)
+    odd = check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 64, 96, 160, None), product_type(cache, q_type))
+    assert odd == nodes * 2 * (7 + 4 + 1 + 64)          # dims of the rows' KV heads, 2 query heads each
