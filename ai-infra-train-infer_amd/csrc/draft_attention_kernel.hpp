@@ -450,7 +450,8 @@ __device__ __forceinline__ void draft_store_stats(const DraftParams& p, const Dr
 }
 
 // The infinities and NaN that tiles of drafted tokens were multiplied without: a row that sees one gets the sum of those
-// it sees in that dim instead of its finite result.  Rare, so it reads V again from the cache, 8 dims of a row per thread.
+// it sees in that dim on top of its result (which earlier tiles may have made infinite or NaN already).  Rare, so it reads V
+// again from the cache, 8 dims of a row per thread.
 template <int KV, int CT, int D, int THREADS>
 __device__ __forceinline__ void draft_wild(const DraftParams& p, const DraftWork& w) {
   constexpr int ES = KV == KV_FP8 ? 1 : 2;
@@ -492,10 +493,11 @@ __device__ __forceinline__ void draft_wild(const DraftParams& p, const DraftWork
     for (int e = 0; e < 8; ++e) {
       if (fabsf(sum[e]) < INFINITY) continue;              // nothing wild in this dim
       if (p.max_partitions == 1) {
-        store_from_f32(p.out, draft_out_at(p, w, r, D) + d + e, p.q_dtype, sum[e]);
+        const int64_t at = draft_out_at(p, w, r, D) + d + e;
+        store_from_f32(p.out, at, p.q_dtype, load_as_f32(p.out, at, p.q_dtype) + sum[e]);
       } else {
         const int64_t at = (((int64_t)w.b * p.nodes + rr / w.gq) * p.num_q_heads + w.kvh * w.gq + rr % w.gq) * p.max_partitions + w.part;
-        p.ws_out[at * D + d + e] = sum[e];
+        p.ws_out[at * D + d + e] += sum[e];
       }
     }
   }

@@ -82,3 +82,15 @@ def test_nan_and_infinity_in_committed_values(pa, gpu, one_width, cache, q_type,
         poison(pool.v, pool.vs, pool.tables, 16, row, pos, head, dims, value)
     odd = check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 64, 96, 160, None), product_type(cache, q_type))
     assert odd == nodes * 2 * (7 + 4 + 1 + 64)          # dims of the rows' KV heads, 2 query heads each
+
+
+@pytest.mark.parametrize("cache,q_type", TYPES)
+def test_nan_and_infinity_in_drafted_and_committed_values(pa, gpu, one_width, cache, q_type):
+    lens, nodes = [90, 64, 0], 9
+    pool, sets, q = random_case(5, lens, nodes, 4, 2, 64, 8, cache, q_type)
+    for row, pos, head, dims, value in ((0, 80, 0, slice(0, 2), float("inf")), (0, 10, 0, slice(2, 3), float("inf")),
+                                        (0, 92, 0, slice(1, 3), -float("inf")),
+                                        (0, 94, 0, slice(4, 9), float("nan")), (1, 40, 1, slice(2, 3), float("nan")),
+                                        (1, 66, 1, slice(20, 40), float("inf")), (2, 3, 0, slice(0, 8), -float("inf"))):
+        poison(pool.v, pool.vs, pool.tables, 8, row, pos, head, dims, value)
+    assert check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 96, None), product_type(cache, q_type)) > 0
