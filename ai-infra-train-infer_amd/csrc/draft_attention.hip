@@ -4,7 +4,8 @@
 namespace pa {
 
 // out = sum_p w_p out_p / sum_p w_p with w_p = sum_p * 2^(max_p - max) over the partitions of a (node, query head) row that
-// hold tokens; a row that saw nothing in any of them is zero, and so is a node that the row does not draft.
+// hold tokens; a partition without a maximum weighs nothing, or NaN if it met a score of NaN.  A row that saw nothing in any of
+// them is zero, and so is a node that the row does not draft.
 // D / 4 threads read one partial result 16 bytes each; `slots` of them side by side take the row's partitions in turn, and
 // 256 / (slots x D / 4) rows share a workgroup: with few partitions a row needs few threads, with many they are read at once.
 // Bound by latency: the maxima and sums, the context length that says how many of them count, and the first partial results
@@ -44,7 +45,8 @@ __global__ __launch_bounds__(kDraftMergeThreads) void draft_merge_kernel(const D
   __syncthreads();
   float top = -INFINITY;
   for (int q = 0; q < np; ++q) top = fmaxf(top, s_max[q]);
-  for (int q = tg; q < np; q += group) s_w[q] = s_max[q] == -INFINITY ? 0.0f : s_w[q] * __builtin_amdgcn_exp2f(s_max[q] - top);
+  for (int q = tg; q < np; q += group)
+    if (s_max[q] != -INFINITY) s_w[q] *= __builtin_amdgcn_exp2f(s_max[q] - top);
   __syncthreads();
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   auto add = [&](int q, const float4& v) __attribute__((always_inline)) {
@@ -65,9 +67,10 @@ __global__ __launch_bounds__(kDraftMergeThreads) void draft_merge_kernel(const D
     const float4 v = s_acc[tid + i * LPP];
     acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
   }
-  const float inv = top == -INFINITY ? 0.0f : 1.0f / den;
+  const float inv = 1.0f / den;
   const int64_t o = (int64_t)bn * p.out_stride + (int64_t)head * D + 4 * ld;
-  const float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  float x[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  if (__builtin_expect(top == -INFINITY, 0)) x[0] = x[1] = x[2] = x[3] = live ? draft_unreferenced(p, b, node) : 0.0f;
   if (p.q_dtype == PA_DTYPE_F32) *(float4*)((float*)p.out + o) = make_float4(x[0], x[1], x[2], x[3]);
   else if (p.q_dtype == PA_DTYPE_F16) *(uint2*)((uint16_t*)p.out + o) = make_uint2(draft_pack<CT_F16>(x[0], x[1]), draft_pack<CT_F16>(x[2], x[3]));
   else *(uint2*)((uint16_t*)p.out + o) = make_uint2(draft_pack<CT_BF16>(x[0], x[1]), draft_pack<CT_BF16>(x[2], x[3]));

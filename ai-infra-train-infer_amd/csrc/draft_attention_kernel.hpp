@@ -19,7 +19,8 @@
 //    [0, 2^8] relative to the reference point.
 //  * The mask is looked at only in tiles that reach the drafted tokens or the end: 32 bits a row, cut out of the
 //    row's mask words.  A row that has seen nothing yet has reference -inf; one that sees nothing at all sums to
-//    zero and its output is zero.
+//    zero and its output is zero.  Scores of NaN never move the reference but make the row's sum NaN, and a row that sees
+//    keys and yet has no reference at the end (all of them NaN or -inf) is NaN, as its softmax is (draft_unreferenced).
 //  * NaN or infinity in the V of a node must not reach the nodes that do not see it, but a matrix product adds
 //    0 * NaN.  Tiles of drafted tokens enter LDS without such values; if there were any, the rows that do see them get
 //    them at the end (draft_wild).
@@ -425,6 +426,18 @@ __device__ __forceinline__ uint32_t draft_visible(const DraftParams& p, const Dr
   return left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1u) : 0u;
 }
 
+// What a row without a reference maximum holds: zero if it sees no key, NaN if what it sees are scores of NaN and -inf alone.
+__device__ __forceinline__ float draft_unreferenced(const DraftParams& p, int b, int node) {
+  bool sees = p.context_lens[b] > 0;
+  const uint64_t* words = p.mask + b * p.mask_stride + (int64_t)node * p.words;
+  const int n = draft_nodes(p, b);
+  for (int i = 0; 64 * i < n; ++i) {
+    const int left = n - 64 * i;
+    sees = sees || (left >= 64 ? words[i] : words[i] & ((1ull << left) - 1)) != 0;
+  }
+  return sees ? __builtin_nanf("") : 0.0f;
+}
+
 // Writes one row's 4 dims of result, or of a partition's partial result.
 __device__ __forceinline__ void draft_store4(const DraftParams& p, const DraftWork& w, int r, int d, int D, const float (&x)[4]) {
   if (p.max_partitions == 1) {
@@ -446,7 +459,7 @@ __device__ __forceinline__ void draft_store_stats(const DraftParams& p, const Dr
   const int rr = w.row0 + r;
   const int64_t at = (((int64_t)w.b * p.nodes + rr / w.gq) * p.num_q_heads + w.kvh * w.gq + rr % w.gq) * p.max_partitions + w.part;
   p.ws_max[at] = top;
-  p.ws_sum[at] = top == -INFINITY ? 0.0f : sum;
+  p.ws_sum[at] = sum;                // without a maximum 0, or NaN if a score was
 }
 
 // The infinities and NaN that tiles of drafted tokens were multiplied without: a row that sees one gets the sum of those
@@ -713,7 +726,12 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
         top = fmaxf(top, sm[16 * c + r][i]);
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = top == -INFINITY ? 0.0f : x[e] / den;   // a row that saw no key: zero
+      for (int e = 0; e < 4; ++e) x[e] = x[e] / den;
+      if (__builtin_expect(top == -INFINITY, 0)) {           // partitions: the merge decides
+        const float none = p.max_partitions > 1 ? 0.0f : draft_unreferenced(p, w.b, (w.row0 + 16 * c + r) / w.gq);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = none;
+      }
       draft_store4(p, w, 16 * c + r, d, D, x);
       if (p.max_partitions > 1 && d == 0) draft_store_stats(p, w, 16 * c + r, top, den);
     }
@@ -932,11 +950,14 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
       const float f1 = t1 == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(t1 - mx);
       const float total = sum[c] * f0 + at[D + 1] * f1;
       if (r >= w.live) continue;
-      const float inv = mx == -INFINITY ? 0.0f : 1.0f / total;               // a row that saw no key: zero
+      const float inv = 1.0f / total;
+      const bool none = mx == -INFINITY;
+      float instead = 0.0f;                                  // partitions: the merge decides
+      if (__builtin_expect(none, 0) && p.max_partitions == 1) instead = draft_unreferenced(p, w.b, (w.row0 + r) / w.gq);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const mfloat4_t v = (rows.o[c][mt] * f0 + *(const mfloat4_t*)(at + 16 * mt + 4 * kg) * f1) * inv;
-        const float x[4] = {v[0], v[1], v[2], v[3]};
+        const float x[4] = {none ? instead : v[0], none ? instead : v[1], none ? instead : v[2], none ? instead : v[3]};
         draft_store4(p, w, r, 16 * mt + 4 * kg, D, x);
       }
       if (p.max_partitions > 1 && kg == 0) draft_store_stats(p, w, r, mx, total);

@@ -557,7 +557,8 @@ int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int6
  * tokens and to the nodes j < num_nodes[b] of its mask, whose K and V lie at cache positions context_lens[b] + j:
  *   out[b, i, h, :] = softmax_j(scale * q[b, i, h, :] . K[b, j, h / G, :]) @ V[b, :, h / G, :]
  * A node that sees nothing (no context and an empty mask), nodes past num_nodes and rows of negative context
- * get zeros.  What a node does not see never reaches its output, NaN and infinities included.
+ * get zeros.  What a node does not see never reaches its output, NaN and infinities included; those of its query and
+ * of what it sees do as the formula has it, however the launch is shaped (scores of nothing but NaN and -inf: NaN).
  *   q, out               [batch, nodes, num_q_heads, head_dim] f16 / bf16 / f32, node stride in elements (rows of
  *                        the batch nodes x stride apart), 16-byte aligned rows (out: 8 bytes do for f16 / bf16)
  *   tree_mask            as pa_draft_layout writes it, rows mask_stride words apart, 0: one tree for every row

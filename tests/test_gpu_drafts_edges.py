@@ -94,3 +94,42 @@ def test_nan_and_infinity_in_drafted_and_committed_values(pa, gpu, one_width, ca
                                         (1, 66, 1, slice(20, 40), float("inf")), (2, 3, 0, slice(0, 8), -float("inf"))):
         poison(pool.v, pool.vs, pool.tables, 8, row, pos, head, dims, value)
     assert check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 96, None), product_type(cache, q_type)) > 0
+
+
+@pytest.mark.parametrize("cache,q_type", TYPES)
+@pytest.mark.parametrize("nodes", [3, 21])
+def test_a_query_with_nan_or_infinity_has_no_finite_output(pa, gpu, one_width, cache, q_type, nodes):
+    """An overflow before the attention must not come out as a vector of zeros, whatever the width and the split; other
+    nodes and heads are as they were."""
+    lens = [130, 0, 65]
+    pool, sets, q = random_case(7, lens, nodes, 4, 2, 64, 16, cache, q_type)
+    q[0, 1, 2, 5] = float("nan")
+    q[1, 0, 0, :] = float("nan")
+    q[2, 2, 3, 63] = float("inf")
+    q[2, 1, 0, 7] = -float("inf")
+    assert check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 96, None), product_type(cache, q_type)) == 4 * 64
+
+
+@pytest.mark.parametrize("cache,q_type", TYPES)
+def test_nan_and_infinity_in_keys(pa, gpu, one_width, cache, q_type):
+    """A NaN key that is all a node sees of its partition, one among others, and (16-bit caches) infinite keys, whose score
+    is an infinity of either sign."""
+    lens, nodes = [64, 96, 33, 0], 4
+    pool, _, q = random_case(9, lens, nodes, 4, 2, 64, 16, cache, q_type)
+    sets = [so.ancestors([-1, 0, 0, 0]) for _ in lens]
+    for row, pos, head, value in ((0, 64, 0, float("nan")), (0, 66, 1, float("nan")), (1, 10, 0, float("nan")),
+                                  (2, 35, 1, float("inf")), (3, 2, 0, -float("inf"))):
+        poison(pool.k, pool.ks, pool.tables, 16, row, pos, head, slice(3, 4), value)
+    assert check_elements(pa, gpu, pool, q, lens, sets, (0, 32, 64, None), product_type(cache, q_type)) > 0
+
+
+@pytest.mark.parametrize("part", [0, 32])
+def test_scores_of_minus_infinity_alone_are_nan_and_no_key_is_zero(pa, gpu, one_width, part):
+    """softmax of nothing but -inf is NaN; a node without any key is the documented zero."""
+    pool, _, q = random_case(11, [0, 0, 40], 3, 2, 1, 64, 16, "fp16", "fp16")
+    q[..., 0] = 1.0
+    for row, pos in ((0, 0), (0, 1), (2, 41)):
+        poison(pool.k, None, pool.tables, 16, row, pos, 0, slice(0, 1), -float("inf"))
+    sets = [[{0}, {0, 1}, set()], [{0}, set(), {2}], [set(), {1}, set()]]
+    odd = check_elements(pa, gpu, pool, q, [0, 0, 40], sets, (part,), torch.float16)
+    assert odd == 2 * 2 * 64          # nodes 0 and 1 of row 0; row 2's node 1 has its committed tokens
