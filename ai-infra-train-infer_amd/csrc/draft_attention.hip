@@ -36,7 +36,8 @@ __global__ __launch_bounds__(kDraftMergeThreads) void draft_merge_kernel(const D
     if (q < np_max) ahead[k] = *(const float4*)(p.ws_out + (at + q) * D + 4 * ld);
   }
   const bool live = node < draft_nodes(p, b);
-  const int np = live ? min((draft_keys(p, b) + p.partition_size - 1) / p.partition_size, np_max) : 0;
+  const int keys = draft_keys(p, b), whole = keys / p.partition_size;       // no rounding up: sizes go up to 2^31 - 256
+  const int np = live ? min(whole + (keys % p.partition_size != 0 ? 1 : 0), np_max) : 0;
   for (int q = tg; q < np_max; q += group) {
     const float m = p.ws_max[at + q], w = p.ws_sum[at + q];
     s_max[q] = q < np ? m : -INFINITY;

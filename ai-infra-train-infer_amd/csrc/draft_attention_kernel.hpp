@@ -391,7 +391,8 @@ __device__ __forceinline__ bool draft_work(const DraftParams& p, DraftWork& w) {
   w.end = keys;
   if (p.max_partitions > 1) {
     w.begin = w.part * p.partition_size;
-    w.end = w.part == p.max_partitions - 1 ? keys : min(w.begin + p.partition_size, keys);
+    // no sum of a place and a size before it is known to stay below the keys
+    w.end = w.part == p.max_partitions - 1 || keys - w.begin <= p.partition_size ? keys : w.begin + p.partition_size;
   }
   return w.live > 0 && w.begin < w.end;
 }

@@ -133,3 +133,27 @@ def test_scores_of_minus_infinity_alone_are_nan_and_no_key_is_zero(pa, gpu, one_
     sets = [[{0}, {0, 1}, set()], [{0}, set(), {2}], [set(), {1}, set()]]
     odd = check_elements(pa, gpu, pool, q, [0, 0, 40], sets, (part,), torch.float16)
     assert odd == 2 * 2 * 64          # nodes 0 and 1 of row 0; row 2's node 1 has its committed tokens
+
+
+# ---------------------------------------------------------------------------------------------- sizes
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_partition_longer_than_any_row(pa, gpu, lib, dim):
+    """The C entry takes partition sizes up to 2^31 - 256: a row then has one partition, whatever its length."""
+    lens, nodes, hq, hkv = [300, 5, 700], 6, 4, 2
+    pool, sets, q = random_case(17, lens, nodes, hq, hkv, dim, 16, "fp16", "fp16")
+    k, v, tables, _, _ = pool.device(gpu)
+    mask = torch.stack([so.mask_words(s, nodes) for s in sets]).to(gpu)
+    qd, lens_t = q.to(gpu), i32(lens, gpu)
+    want = pa.paged_draft_attention(qd, k, v, tables, lens_t, mask, dim ** -0.5, partition_size=0)
+    need = lib.pa_draft_workspace_bytes(3, nodes, hq, dim, 2)
+    ws = torch.empty(need, dtype=torch.uint8, device=gpu)
+    for size in (0x7fffff00, 1 << 30, 1024):
+        out = torch.full_like(qd, 9.0)
+        rc = lib.pa_draft_attention(qd.data_ptr(), 0, hq * dim, k.data_ptr(), v.data_ptr(), None, None, 0, tables.data_ptr(),
+                                    tables.stride(0), tables.shape[1], lens_t.data_ptr(), None, mask.data_ptr(), mask[0].numel(),
+                                    out.data_ptr(), hq * dim, 3, nodes, hq, hkv, dim, 16, pool.blocks, dim ** -0.5, size, 2,
+                                    ws.data_ptr(), need, 0, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0, lib.pa_last_error()
+        # one partition in both: the merge multiplies and divides by its sum, then rounds the same value
+        torch.testing.assert_close(out.float(), want.float(), rtol=2.0 ** -10, atol=2.0 ** -20)
