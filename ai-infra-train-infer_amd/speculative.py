@@ -361,6 +361,8 @@ def commit_drafts(kv_cache, block_tables, context_lens, path, counts, k_scale=No
         raise RuntimeError("%s: kv_cache must be contiguous [2, layers, num_blocks, block_size, kv_heads, head_dim]" % what)
     lib = _native.load()
     _, layers, num_blocks, block_size, heads, head_dim = kv_cache.shape
+    if layers == 0:      # the launch that moves the rows of the layers writes the lengths, too
+        raise RuntimeError("%s: a pool without layers" % what)
     lens = _int32(context_lens, what)
     if lens.dim() != 1:
         lens = lens.view(-1)

@@ -543,7 +543,7 @@ int pa_verify_drafts(const void* logits, int dtype, int64_t row_stride, int64_t 
  *                        planes plane_stride_bytes apart
  *   k_scale, v_scale     fp8 pools: [layers][num_blocks][block_size] float, layers scale_stride apart; else NULL
  *   path, counts         as pa_verify_drafts writes them: ascending nodes, so that path[j] >= j
- *   new_lens             int32 [batch], not context_lens itself
+ *   new_lens             int32 [batch], not context_lens itself; not written where layers is 0: there is nothing to do
  * Positions outside a row's table or the pool are skipped.  The rows' drafted positions must not share blocks.
  */
 int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int64_t row_bytes, float* k_scale,

@@ -157,3 +157,12 @@ def test_a_partition_longer_than_any_row(pa, gpu, lib, dim):
         assert rc == 0, lib.pa_last_error()
         # one partition in both: the merge multiplies and divides by its sum, then rounds the same value
         torch.testing.assert_close(out.float(), want.float(), rtol=2.0 ** -10, atol=2.0 ** -20)
+
+
+@pytest.mark.parametrize("cache", ["fp16", "fp8"])
+def test_commit_refuses_a_pool_without_layers(pa, gpu, cache):
+    kv = torch.zeros(2, 0, 4, 8, 1, 64, device=gpu).to(DT[cache])
+    lens, path = i32([3, 4], gpu), torch.zeros(2, 3, dtype=torch.int32, device=gpu)
+    scales = [torch.zeros(0, 4, 8, device=gpu)] * 2 if cache == "fp8" else []
+    with pytest.raises(RuntimeError, match="layer"):
+        pa.commit_drafts(kv, torch.zeros(2, 2, dtype=torch.int32, device=gpu), lens, path, i32([1, 1], gpu), *scales)
