@@ -121,7 +121,7 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
         return positions, slots, mask
     rc = lib.pa_draft_layout(parents.data_ptr(), stride, lens.data_ptr(), real.data_ptr() if real is not None else None,
                              tables_ptr, row, width, positions.data_ptr(), slots_ptr, mask.data_ptr(), batch, nodes,
-                             int(block_size), int(num_blocks or 1), _stream_ptr(device))
+                             int(block_size), 1 if num_blocks is None else int(num_blocks), _stream_ptr(device))
     _native.check(rc, "pa_draft_layout")
     return positions, slots, mask
 

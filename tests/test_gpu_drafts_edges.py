@@ -166,3 +166,8 @@ def test_commit_refuses_a_pool_without_layers(pa, gpu, cache):
     scales = [torch.zeros(0, 4, 8, device=gpu)] * 2 if cache == "fp8" else []
     with pytest.raises(RuntimeError, match="layer"):
         pa.commit_drafts(kv, torch.zeros(2, 2, dtype=torch.int32, device=gpu), lens, path, i32([1, 1], gpu), *scales)
+
+
+def test_layout_refuses_a_pool_without_blocks(pa, gpu):
+    with pytest.raises(RuntimeError, match="pool"):
+        pa.draft_layout(i32([-1, 0], gpu), i32([3], gpu), torch.zeros(1, 4, dtype=torch.int32, device=gpu), 16, 0)
