@@ -217,6 +217,8 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
     if flat.data_ptr() % 16:
         flat, q_stride = flat.clone(memory_format=torch.contiguous_format), num_q_heads * head_dim
     tables, tables_row, width = _tables(block_tables, batch, what)
+    if width == 0:
+        raise RuntimeError("%s: block_tables without columns" % what)
     lens = _int32(context_lens, what)
     real = _lengths(num_nodes, batch, "num_nodes", what)
     mask = tree_mask.contiguous()
@@ -241,7 +243,7 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
                                "than the table's %d columns" % (what, bad, num_blocks, short, width))
     if partition_size is None:
         bound = width * block_size
-        if longest_context:
+        if longest_context and longest_context > 0:
             bound = min(bound, -(-(int(longest_context) + nodes) // 256) * 256)
         # sixteenths of the bound: batches of about the same shape share the decision
         mean = bound if not mean_context else max(1, min(16, round(16.0 * (mean_context + nodes) / bound))) * bound // 16

@@ -171,3 +171,19 @@ def test_commit_refuses_a_pool_without_layers(pa, gpu, cache):
 def test_layout_refuses_a_pool_without_blocks(pa, gpu):
     with pytest.raises(RuntimeError, match="pool"):
         pa.draft_layout(i32([-1, 0], gpu), i32([3], gpu), torch.zeros(1, 4, dtype=torch.int32, device=gpu), 16, 0)
+
+
+def test_attention_refuses_a_table_without_columns_and_takes_any_hint(pa, gpu):
+    pool, sets, q = random_case(19, [40, 3], 3, 4, 2, 64, 16, "fp16", "fp16")
+    k, v, tables, _, _ = pool.device(gpu)
+    mask = torch.stack([so.mask_words(s, 3) for s in sets]).to(gpu)
+    call = lambda t, **kw: pa.paged_draft_attention(q.to(gpu), k, v, t, i32([40, 3], gpu), mask, 0.125, **kw)
+    for part in (None, 0, 32):
+        with pytest.raises(RuntimeError, match="block_tables"):
+            call(tables[:, :0], partition_size=part)
+    want = call(tables, partition_size=0)
+    # two roundings of the probabilities (bound()'s 2^-11 + 2^-13 of the values' size each) and of the output
+    far = 2 * (2.0 ** -11 + 2.0 ** -13) * float(pool.vf.abs().max())
+    for longest, mean in ((-3, None), (-400, -7.0), (1, 1.0), (1 << 40, 1e12), (5, 1e9)):
+        torch.testing.assert_close(call(tables, longest_context=longest, mean_context=mean).float(), want.float(),
+                                   rtol=2.0 ** -10, atol=far)
