@@ -217,8 +217,6 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
     if flat.data_ptr() % 16:
         flat, q_stride = flat.clone(memory_format=torch.contiguous_format), num_q_heads * head_dim
     tables, tables_row, width = _tables(block_tables, batch, what)
-    if width == 0:
-        raise RuntimeError("%s: block_tables without columns" % what)
     lens = _int32(context_lens, what)
     real = _lengths(num_nodes, batch, "num_nodes", what)
     mask = tree_mask.contiguous()
@@ -228,6 +226,8 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
         raise RuntimeError("%s: out must be contiguous and like q" % what)
     if batch == 0:
         return out
+    if width == 0:
+        raise RuntimeError("%s: block_tables without columns" % what)
     kv_code = _code(k_cache.dtype, what)
     scales = (None, None)
     fp8 = kv_code == _native.DTYPE_FP8_E4M3

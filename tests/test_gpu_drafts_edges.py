@@ -181,6 +181,8 @@ def test_attention_refuses_a_table_without_columns_and_takes_any_hint(pa, gpu):
     for part in (None, 0, 32):
         with pytest.raises(RuntimeError, match="block_tables"):
             call(tables[:, :0], partition_size=part)
+    empty = pa.paged_draft_attention(q[:0].to(gpu), k, v, tables[:0, :0], i32([], gpu), mask[:1], 0.125)
+    assert empty.shape == (0, 3, 4, 64)           # no rows, no table
     want = call(tables, partition_size=0)
     # two roundings of the probabilities (bound()'s 2^-11 + 2^-13 of the values' size each) and of the output
     far = 2 * (2.0 ** -11 + 2.0 ** -13) * float(pool.vf.abs().max())
