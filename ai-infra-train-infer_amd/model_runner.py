@@ -751,7 +751,8 @@ class ModelRunner:
         the last accepted token), parents int32 [nodes] or [batch, nodes], block_tables [batch, max_blocks] int32 that
         reach context_len + nodes, context_lens [batch] int32 (committed tokens), num_nodes int32 [batch] or None ->
         logits [batch, nodes, vocab], the distribution after every node.  Node i's K and V are written at cache
-        position context_len + i of every layer.  longest_context / mean_context: what the host knows of context_lens."""
+        position context_len + i of every layer.  longest_context / mean_context: what the host knows of context_lens.
+        Ids past num_nodes can be anything (their logits mean nothing), the others belong to the vocabulary."""
         from .speculative import draft_layout
         if self.model is None:
             raise RuntimeError("run_drafts: the runner has no model of PagedAttention layers")
@@ -762,7 +763,9 @@ class ModelRunner:
         set_context(is_prefill=False, slot_mapping=slots.view(-1), context_lens=context_lens, block_tables=block_tables,
                     longest_context_len=longest_context, mean_context_len=mean_context, tree_mask=mask, num_nodes=num_nodes)
         try:
-            logits = self.model(tokens.reshape(-1), positions=positions.view(-1))
+            # a node without a slot is none of its row's: whatever id stands there (-1 in verify_drafts' padding) must not reach
+            # the embedding, which reads its table at any id it gets
+            logits = self.model(tokens.masked_fill(slots < 0, 0).reshape(-1), positions=positions.view(-1))
         finally:
             reset_context()
         return logits.view(*tokens.shape, -1)

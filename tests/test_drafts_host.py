@@ -185,3 +185,36 @@ def test_run_drafts_refuses_a_runner_without_a_model(pa):
     one = torch.zeros(1, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="no model"):
         runner.run_drafts(one.long(), one, one, one[0])
+
+
+@pytest.mark.parametrize("shared", [False, True])
+def test_run_drafts_asks_the_model_for_no_id_behind_a_rows_nodes(pa, monkeypatch, shared):
+    """verify_drafts pads its tokens with -1, and a padded row's ids can be anything: nodes without a slot must not reach the
+    embedding, which reads its table at whatever id it gets."""
+    from ai_infra_train_infer_amd import speculative
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.embed = torch.nn.Embedding(10, 4)
+
+        def forward(self, ids, positions):
+            self.ids = ids
+            return self.embed(ids)
+
+    def layout(parents, context_lens, tables, block_size, num_blocks, num_nodes):
+        pos, slots = zip(*[so.layout(parents.tolist() if parents.dim() == 1 else parents[b].tolist(), int(context_lens[b]),
+                                     int(num_nodes[b]) if context_lens[b] >= 0 else 0, tables[b].tolist(), block_size, num_blocks)[:2]
+                           for b in range(len(context_lens))])
+        return torch.tensor(pos), torch.tensor(slots, dtype=torch.int32), torch.zeros(1, 3, 1, dtype=torch.int64)
+
+    monkeypatch.setattr(speculative, "draft_layout", layout)
+    model = Model()
+    runner = pa.ModelRunner(model, pa.ModelRunnerConfig(block_size=16, device="cpu"))
+    tokens = torch.tensor([[3, -1, 5, 10], [9, 1 << 40, 6, 4], [-1, -7, 7, 4]]).t()       # in any order in memory
+    kept = tokens.clone()
+    parents = torch.tensor([-1, 0, 0], dtype=torch.int32)
+    logits = runner.run_drafts(tokens, parents if shared else parents.expand(4, 3).contiguous(), torch.zeros(4, 2, dtype=torch.int32),
+                               torch.tensor([4, 4, 4, -1], dtype=torch.int32), num_nodes=torch.tensor([2, 0, 3, 3], dtype=torch.int32))
+    assert logits.shape == (4, 3, 4) and torch.equal(tokens, kept)
+    assert model.ids.tolist() == [3, 9, 0, 0, 0, 0, 5, 6, 7, 0, 0, 0]

@@ -271,3 +271,30 @@ def test_a_capture_whose_workspace_was_not_reserved_raises(pa, gpu):
         attention._WORKSPACES.update(kept)
     torch.cuda.synchronize()
     assert pa.verify_drafts(logits, toks, temperature=0.0)[1].min() >= 1
+
+
+@pytest.mark.parametrize("pad", [-1, 1 << 40])
+def test_padding_ids_never_reach_the_model(pa, gpu, pad):
+    """Ids behind a row's nodes that no vocabulary holds, as verify_drafts writes them: the other rows' logits and the cache
+    are those of a step padded with ordinary ids."""
+    rng = random.Random(13)
+    model = small_model(pa)
+    sess = Speculating(pa, model, gpu)
+    sess.start([[rng.randrange(512) for _ in range(n)] for n in (20, 33, 5)])
+    nodes, real = 6, [6, 0, 3]
+    par, num = i32([make_parents("tree", nodes, rng) for _ in real], gpu), i32(real, gpu)
+    tables, ctx = sess.tables(nodes, gpu), i32(sess.lens(), gpu)
+    toks = torch.tensor([[rng.randrange(512) for _ in range(nodes)] for _ in real], device=gpu)
+    odd = toks.clone()
+    for b, n in enumerate(real):
+        odd[b, n:] = pad
+        toks[b, n:] = 0
+    cache = sess.pool.kv_cache_tensor
+    before = cache.clone()
+    want = sess.runner.run_drafts(toks, par, tables, ctx, num_nodes=num)
+    after = cache.clone()
+    cache.copy_(before)
+    got = sess.runner.run_drafts(odd, par, tables, ctx, num_nodes=num)
+    assert torch.equal(cache, after) and got.shape == want.shape
+    for b, n in enumerate(real):
+        assert torch.equal(got[b, :n], want[b, :n])
