@@ -529,7 +529,8 @@ __global__ __launch_bounds__(kStatThreads) void draft_row_argmax_kernel(const Ve
   __syncthreads();
   if (tid == 0) {
     for (int w = 0; w < kStatWaves; ++w) take(redi[w], redv[w]);
-    p.cut[(int64_t)b * p.nodes + node] = __int_as_float(best_i < p.vocab ? best_i : 0);
+    // without a maximum above -inf: a NaN before the first -inf counts as one, too
+    p.cut[(int64_t)b * p.nodes + node] = __int_as_float(best > -INFINITY ? best_i : 0);
   }
 }
 

@@ -189,3 +189,18 @@ def test_attention_refuses_a_table_without_columns_and_takes_any_hint(pa, gpu):
     for longest, mean in ((-3, None), (-400, -7.0), (1, 1.0), (1 << 40, 1e12), (5, 1e9)):
         torch.testing.assert_close(call(tables, longest_context=longest, mean_context=mean).float(), want.float(),
                                    rtol=2.0 ** -10, atol=far)
+
+
+# ---------------------------------------------------------------------------------------------- verification
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+def test_greedy_without_a_finite_logit_takes_the_first_token(pa, gpu, dtype):
+    """NaN counts as -inf, so the first maximum of a row of both is its first entry."""
+    def none(x):
+        x[0] = -float("inf")
+        x[0, :, :3] = float("nan")
+        x[1] = float("nan")
+        x[1, :, 40:] = -float("inf")
+        x[2] = -float("inf")
+        x[3, :, :100] = float("nan")
+    check_verify(pa, gpu, 71, 5, 4, 200, dtype, 0.0, 1.0, change=none)
