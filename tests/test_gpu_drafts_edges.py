@@ -204,3 +204,16 @@ def test_greedy_without_a_finite_logit_takes_the_first_token(pa, gpu, dtype):
         x[2] = -float("inf")
         x[3, :, :100] = float("nan")
     check_verify(pa, gpu, 71, 5, 4, 200, dtype, 0.0, 1.0, change=none)
+
+
+def test_row_sums_of_large_vocabularies_of_32_bit_logits(pa, gpu):
+    """4 million entries of 2^-39.99 beside one of 1: they weigh 1.007 * 2^-18 together, and a token of weight 1 passes iff
+    u < 1 / (1 + 1.007 * 2^-18).  Numbers on either side of that, about 2^-19 away."""
+    vocab = 1 << 22
+    logits = torch.full((2, 2, vocab), -39.99 * math.log(2.0), device=gpu)
+    logits[:, :, 5] = 0.0
+    u = torch.tensor([[0.0, 1 - 1.5 * 2.0 ** -18], [0.0, 1 - 0.5 * 2.0 ** -18]], device=gpu)
+    tokens = torch.full((2, 2), 5, device=gpu)
+    for top_p in (1 - 2.0 ** -20, 1.0):
+        _, counts, _ = pa.verify_drafts(logits, tokens, u, temperature=1.0, top_p=top_p)
+        assert counts.tolist() == [2, 1], top_p
