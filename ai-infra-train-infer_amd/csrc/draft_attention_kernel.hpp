@@ -14,7 +14,8 @@
 //    (16 bytes per lane), written to LDS, S^T = K . Q^T and O^T += V^T . P^T with 16x16x32 products, V^T through the
 //    LDS transpose read.
 //  * Queries keep their own bits (no scale folded in): 16-bit caches and queries of one type are multiplied as
-//    they are, everything else as fp16, and scale * log2(e) is applied to the fp32 score in the same fused
+//    they are, everything else as fp16, bf16 and fp32 queries times a power of two per row that brings their largest
+//    element to fp16's range.  scale * log2(e), and that power, are applied to the fp32 score in the same fused
 //    multiply-add that subtracts the reference maximum.  What is rounded to 16 bits is the probability, in
 //    [0, 2^8] relative to the reference point.
 //  * The mask is looked at only in tiles that reach the drafted tokens or the end: 32 bits a row, cut out of the
@@ -198,6 +199,7 @@ struct DraftRows {
   static constexpr int KSTEPS = D / 32, MT = D / 16, ROWB = D * 2, CPR = D / 8;
   mword4_t q[C][KSTEPS];         // Q^T as the B operand: dims 32 s + 8 kg .. + 7 of row 16 c + col
   mfloat4_t o[C][MT];
+  float scale[C];                // what a product is times to be a score in log2 units
   float m_ref[C];                // reference maximum in log2 units, the same in a row's 4 lanes; -inf: nothing seen
   float l_run[C];                // this lane's share of the row's sum
   uint32_t k_first, v_first;     // this lane's K fragment of dims 0 .. 31 and V fragment of dims 0 .. 15 in a tile
@@ -221,24 +223,47 @@ struct DraftRows {
 
   // at(c): element index of row 16 c + col's query
   template <class At>
-  __device__ __forceinline__ void load_q(const void* ptr, int dtype, At&& at) {
+  __device__ __forceinline__ void load_q(const void* ptr, int dtype, float scale_log2e, At&& at) {
     // the dtype switch sits outside the loops: inside, it would put a branch and a wait between loads in flight
     auto load = [&](auto dt_tag) __attribute__((always_inline)) {
+      constexpr int DT = decltype(dt_tag)::value;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int64_t base = at(c) + 8 * kg;
+        float x[KSTEPS][8];
 #pragma unroll
-        for (int s = 0; s < KSTEPS; ++s) {
-          float x[8];
-          load8_as_f32(ptr, base + 32 * s, decltype(dt_tag)::value, x);
+        for (int s = 0; s < KSTEPS; ++s) load8_as_f32(ptr, base + 32 * s, DT, x[s]);
+        scale[c] = scale_log2e;
+        if constexpr (CT == CT_F16 && DT != PA_DTYPE_F16) {
+          // the row's largest element to 2^14 ... 2^15: no size overflows, and what is more than 2^28 below it alone loses bits
+          float most = 0.0f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q[c][s][e] = draft_pack<CT>(x[2 * e], x[2 * e + 1]);
+          for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[s][e]));
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          // nothing to bring anywhere in a row of zeros, and none that would help one of infinities
+          const int up = most > 0.0f && most < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(most), 100) : 0;
+          scale[c] = __builtin_amdgcn_ldexpf(scale_log2e, -up);
+#pragma unroll
+          for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[s][e] = __builtin_amdgcn_ldexpf(x[s][e], up);
         }
+#pragma unroll
+        for (int s = 0; s < KSTEPS; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[c][s][e] = draft_pack<CT>(x[s][2 * e], x[s][2 * e + 1]);
       }
     };
-    if (dtype == PA_DTYPE_F16) load(std::integral_constant<int, PA_DTYPE_F16>{});
-    else if (dtype == PA_DTYPE_BF16) load(std::integral_constant<int, PA_DTYPE_BF16>{});
-    else load(std::integral_constant<int, PA_DTYPE_F32>{});
+    if constexpr (CT == CT_BF16) {
+      load(std::integral_constant<int, PA_DTYPE_BF16>{});
+    } else {
+      if (dtype == PA_DTYPE_F16) load(std::integral_constant<int, PA_DTYPE_F16>{});
+      else if (dtype == PA_DTYPE_BF16) load(std::integral_constant<int, PA_DTYPE_BF16>{});
+      else load(std::integral_constant<int, PA_DTYPE_F32>{});
+    }
   }
 
   // Fragments of a 32-token tile at `tile` (of 256 bytes' alignment: a 16-byte piece's number is exclusive-ored with the row's
@@ -259,8 +284,8 @@ struct DraftRows {
   // k, v: the tile in LDS; iks, mvs: per token 1 / k_scale and the mantissa of 1 / v_scale (fp8).  visible(c): bit k =
   // the row sees key k, asked for only in special tiles.
   template <class Visible>
-  __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, const float* iks, const float* mvs_lds, float scale_log2e,
-                                       bool special, Visible&& visible) {
+  __device__ __forceinline__ void step(const uint8_t* k, const uint8_t* v, const float* iks, const float* mvs_lds, bool special,
+                                       Visible&& visible) {
     mfloat4_t s[C][2];
 #pragma unroll
     for (int c = 0; c < C; ++c)
@@ -312,7 +337,7 @@ struct DraftRows {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[c][kb][e]);
-      top[c] = mx * scale_log2e;                           // scale > 0
+      top[c] = mx * scale[c];                              // scale > 0
       want = want || top[c] > m_ref[c] + 8.0f;
     }
     // The reference follows a row's maximum only when that has outgrown it by 2^8: p <= 256 fits the 16-bit types,
@@ -342,8 +367,8 @@ struct DraftRows {
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-          float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e], scale_log2e, -ref));
-          float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e + 1], scale_log2e, -ref));
+          float p0 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e], scale[c], -ref));
+          float p1 = __builtin_amdgcn_exp2f(fmaf(s[c][kb][e + 1], scale[c], -ref));
           psum += p0 + p1;
           if constexpr (KV == KV_FP8) { p0 *= mvs[kb][e]; p1 *= mvs[kb][e + 1]; }
           pb[c][2 * kb + e / 2] = draft_pack<CT>(p0, p1);
@@ -675,7 +700,7 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
       load_ids(wave, ids);
       issue_as(stream_tag, t, wave, ids);
       // The queries while the first tile is on its way.  Rows without a node repeat the last one; they are never written.
-      rows.load_q(p.q, p.q_dtype, [&](int c) {
+      rows.load_q(p.q, p.q_dtype, p.scale_log2e, [&](int c) {
         const int r = w.row0 + min(16 * c + col, w.live - 1);
         return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
       });
@@ -687,7 +712,7 @@ __global__ __launch_bounds__(kDraftWaves * 64, 2) void draft_narrow_kernel(const
         load_ids(tile + 2 * W, ids_next);
         write_tile(t, tile, special);
         if (i + 1 < n_mine) issue_as(stream_tag, t, tile + W, ids);
-        rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, p.scale_log2e, special, [&](int c) { return draft_visible(p, w, 16 * c + col, first); });
+        rows.step(my_lds, my_lds + draft_half_bytes(D), my_scales, my_scales + TILE, special, [&](int c) { return draft_visible(p, w, 16 * c + col, first); });
 #pragma unroll
         for (int x = 0; x < 4; ++x) ids[x] = ids_next[x];
       }
@@ -894,7 +919,7 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
     const uint8_t* kt = draft_lds + (tile & 1) * 2 * TILEB;
     const float* sc = scales + (tile & 1) * 2 * TK;
     const bool special = first + 32 > w.ctx || first + 32 > end;       // drafted tokens or the end inside
-    rows.step(kt + at * ROWB, kt + TILEB + at * ROWB, sc + at, sc + TK + at, p.scale_log2e, special,
+    rows.step(kt + at * ROWB, kt + TILEB + at * ROWB, sc + at, sc + TK + at, special,
               [&](int c) { return draft_visible(p, w, row_w + 16 * c + col, first); });
   };
 
@@ -903,7 +928,7 @@ __global__ __launch_bounds__(draft_wide_waves(WR) * 64, 2) void draft_wide_kerne
 #pragma unroll
   for (int d = 0; d < DEPTH; ++d) issue(st[d], d);
   // the queries while the first tiles are on their way
-  rows.load_q(p.q, p.q_dtype, [&](int c) {
+  rows.load_q(p.q, p.q_dtype, p.scale_log2e, [&](int c) {
     const int r = w.row0 + min(row_w + 16 * c + col, w.live - 1);
     return ((int64_t)w.b * p.nodes + r / w.gq) * p.q_stride + (int64_t)(w.kvh * w.gq + r % w.gq) * D;
   });

@@ -569,7 +569,9 @@ int pa_draft_commit(void* pool, int64_t layers, int64_t plane_stride_bytes, int6
  *   rows_per_workgroup   (node, query head) rows of one KV head that a workgroup serves from one pass over K and
  *                        V: 16, 32, 64, 128, or 0 = the launch's own choice; never changes what is computed
  * Cache, tables, scales and sizes as for pa_decode.  16-bit caches and queries of one type are multiplied as they
- * are, everything else as fp16; accumulation and softmax statistics are fp32.
+ * are, everything else as fp16: bf16 and f32 queries of any size, since a row is brought to fp16's range by a power of
+ * two; K and V of a bf16 cache as they are (as in pa_decode), so that they count as infinite beyond 65504 there.
+ * Accumulation and softmax statistics are fp32, probabilities are rounded to the type of the products.
  */
 int64_t pa_draft_workspace_bytes(int64_t batch, int64_t nodes, int64_t num_q_heads, int64_t head_dim,
                                  int64_t max_partitions);

@@ -135,6 +135,21 @@ def test_scores_of_minus_infinity_alone_are_nan_and_no_key_is_zero(pa, gpu, one_
     assert odd == 2 * 2 * 64          # nodes 0 and 1 of row 0; row 2's node 1 has its committed tokens
 
 
+# ---------------------------------------------------------------------------------------------- queries of another type
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "bf16"), ("fp16", "fp32"), ("fp8", "bf16"), ("fp8", "fp32"), ("bf16", "fp32")])
+@pytest.mark.parametrize("size", [2.0 ** 40, 2.0 ** 18, 2.0 ** -18, 2.0 ** -40])
+def test_queries_beyond_the_range_of_fp16(pa, gpu, one_width, cache, q_type, size):
+    """Queries of any size that their type holds, the scale taking it back; rows of several sizes side by side."""
+    lens, nodes = [40, 0, 100], 11
+    pool, sets, q = random_case(13, lens, nodes, 4, 2, 64, 16, cache, q_type)
+    q *= size
+    q[:, 3] *= 2.0 ** -9              # its scores all but vanish
+    q[0, 2, 1] = 0.0
+    q[:, 5, :, ::2] *= 2.0 ** -12     # small next to large
+    check_elements(pa, gpu, pool, q, lens, sets, (0, 32), product_type(cache, q_type), scale=64 ** -0.5 / size)
+
+
 # ---------------------------------------------------------------------------------------------- sizes
 
 @pytest.mark.parametrize("dim", [64, 128])
