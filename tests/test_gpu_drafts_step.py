@@ -298,3 +298,65 @@ def test_padding_ids_never_reach_the_model(pa, gpu, pad):
     assert torch.equal(cache, after) and got.shape == want.shape
     for b, n in enumerate(real):
         assert torch.equal(got[b, :n], want[b, :n])
+
+
+@pytest.mark.parametrize("cache_dtype", ["fp16", "fp8"])
+def test_a_captured_steps_cache_is_that_of_its_own_path(pa, gpu, cache_dtype):
+    """After a replay the cache holds, bit for bit, what was there but in the places of the drafted nodes, and in these the rows
+    of an eager forward committed along the replay's own path and counts (fp16: as close as two forwards are; their products
+    may be cut differently)."""
+    from ai_infra_train_infer_amd.attention import sizing_graph_workspace
+    rng = random.Random(17)
+    model = small_model(pa, cache_dtype)
+    sess = Speculating(pa, model, gpu, cache_dtype=cache_dtype)
+    sess.start([[rng.randrange(512) for _ in range(n)] for n in (30, 9, 50, 3)])
+    nodes = 10
+    tables, ctx = sess.tables(nodes, gpu), i32(sess.lens(), gpu)
+    toks = torch.zeros(4, nodes, dtype=torch.int64, device=gpu)
+    par, num = i32([make_parents("tree", nodes, rng) for _ in range(4)], gpu), i32([nodes] * 4, gpu)
+    cache = sess.pool.kv_cache_tensor
+
+    def step():
+        logits = sess.runner.run_drafts(toks, par, tables, ctx, num_nodes=num)
+        out = pa.verify_drafts(logits, toks, parents=par, num_nodes=num, temperature=0.0)
+        return (*out, sess.pool.commit_drafts(tables, ctx, out[2], out[1]))
+
+    start = cache.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), sizing_graph_workspace():
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    kept = 0
+    for replay in range(4):
+        torch.cuda.synchronize()
+        par.copy_(torch.tensor([make_parents(rng.choice(["tree", "deep", "star"]), nodes, rng) for _ in range(4)]))
+        num.copy_(torch.tensor([nodes, rng.randrange(nodes + 1), 4, nodes]))
+        toks.copy_(torch.tensor([[rng.randrange(512) for _ in range(nodes)] for _ in range(4)]))
+        cache.copy_(start)
+        first = sess.runner.run_drafts(toks, par, tables, ctx, num_nodes=num).float()
+        for b in range(4):                                 # the last child of the root is the target's choice
+            children = [c for c in range(1, nodes) if int(par[b, c]) == 0]
+            toks[b, children[-1]] = int(first[b, 0].argmax())
+        cache.copy_(start)
+        graph.replay()
+        torch.cuda.synchronize()
+        got, (out, counts, path, after) = cache.clone(), (t.clone() for t in held)
+        kept += int((counts - 1).clamp(min=0).sum())
+        cache.copy_(start)
+        sess.runner.run_drafts(toks, par, tables, ctx, num_nodes=num)
+        assert torch.equal(sess.pool.commit_drafts(tables, ctx, path, counts), after) and torch.equal(after, ctx + counts)
+        drafted = torch.zeros(cache.shape[2:4], dtype=torch.bool, device=gpu)
+        for b in range(4):
+            for i in range(int(num[b])):
+                p = int(ctx[b]) + i
+                drafted[tables[b, p // 16], p % 16] = True
+        for x in (got, cache):
+            assert torch.equal(x.view(torch.uint8).view(*x.shape[:4], -1)[:, :, ~drafted],
+                               start.view(torch.uint8).view(*x.shape[:4], -1)[:, :, ~drafted])
+        if cache_dtype == "fp16":
+            torch.testing.assert_close(got[:, :, drafted].float(), cache[:, :, drafted].float(), rtol=2e-2, atol=2e-2)
+    assert kept >= 6        # paths of more than the root were committed
