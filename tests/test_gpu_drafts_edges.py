@@ -232,3 +232,30 @@ def test_row_sums_of_large_vocabularies_of_32_bit_logits(pa, gpu):
     for top_p in (1 - 2.0 ** -20, 1.0):
         _, counts, _ = pa.verify_drafts(logits, tokens, u, temperature=1.0, top_p=top_p)
         assert counts.tolist() == [2, 1], top_p
+
+
+# ---------------------------------------------------------------------------------------------- again and again
+
+@pytest.mark.parametrize("cache,q_type", TYPES)
+@pytest.mark.parametrize("part", [None, 0, 96])
+def test_attention_gives_the_same_bits_every_time(pa, gpu, one_width, cache, q_type, part):
+    lens, nodes = [500, 33, 0, 260], 19
+    pool, sets, q = random_case(23, lens, nodes, 8, 2, 128, 16, cache, q_type)
+    k, v, tables, ks, vs = pool.device(gpu)
+    mask = torch.stack([so.mask_words(s, nodes) for s in sets]).to(gpu)
+    call = lambda: pa.paged_draft_attention(q.to(gpu), k, v, tables, i32(lens, gpu), mask, 128 ** -0.5, ks, vs, partition_size=part)
+    first = call()
+    assert all(torch.equal(call(), first) for _ in range(10))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("top_p", [0.9, 1.0])
+def test_verification_gives_the_same_tokens_every_time(pa, gpu, dtype, top_p):
+    g = torch.Generator(device=gpu).manual_seed(29)
+    logits = (torch.randn(16, 12, 20011, generator=g, device=gpu) * 2).to(DT[dtype])
+    tokens = logits[:, 0].float().topk(12).indices
+    u, par = torch.rand(16, 12, generator=g, device=gpu), i32([-1] + [0] * 7 + [1, 2, 3, 4], gpu)
+    call = lambda: pa.verify_drafts(logits, tokens, u, par, temperature=0.9, top_p=top_p)
+    first = call()
+    for _ in range(10):
+        assert all(torch.equal(x, y) for x, y in zip(call(), first))
