@@ -983,11 +983,10 @@ extern "C" int pa_verify_drafts(const void* logits, int dtype, int64_t row_strid
   p.nodes = (int)nodes;
   p.vocab = (int)vocab;
   p.chunks = (int)((vocab + kChunk - 1) / kChunk);
-  // With draft probabilities a wave's chunks are a long chain of loads, exponentials and sums: as many workgroups as the GPU
-  // holds at once, six a CU (64 rows of 152k entries: 27 us with 1536 workgroups, 34 with 512,
-  // before an exponential lost a third of its instructions; 21 now).  Without, the walk that every
-  // workgroup repeats weighs more: half of that (16 rows of 64 nodes: 11 us with 512, 12 with 1024, 14 with 1536).
-  const int64_t want = ((p.q ? 1536 : 768) + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
+  // A wave's chunks are a long chain of loads, exponentials and sums: as many workgroups as the GPU holds at once, six a CU, though
+  // each of a row repeats its walk.  The whole call with 1536, 768 and 512 of them, rows of 152k entries: 64 chains of 5 with draft
+  // probabilities 48, 51 and 56 us; 64 trees of 8 nodes 75, 78 and 82; 16 trees of 64 nodes 113, 113 and 114.
+  const int64_t want = (1536 + batch - 1) / batch, most = (p.chunks + kWalkWaves - 1) / kWalkWaves;
   p.slices = (int)(want < most ? want : most);
   p.z = (double*)(ws + l.z);
   p.top = (float*)(ws + l.top);
