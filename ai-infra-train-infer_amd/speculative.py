@@ -132,9 +132,11 @@ def draft_layout(parents, context_lens, block_tables=None, block_size=16, num_bl
 # the bytes per ns that a launch of them draws from HBM.  A launch lasts as long as its rounds of workgroups and the memory
 # need, neither quite hidden behind the other; a split adds the merge pass and the partial results it writes and reads.
 # Fitted to a sweep of tiles and splits on an MI355X (19 shapes: batch 1 to 64, 5 to 64 nodes, 512 to 32k tokens, ratios of 2
-# to 8, head_dim 128, fp16, bf16 and fp8 caches, K and V cold): the choice is within 1 % of the sweep's best on average, 7 % at
-# worst.  Wide workgroups pay also where they are half empty, since they have the most loads in flight: 24 rows of 10 nodes x 4
-# query heads a KV head x 3000 tokens take 58 us with 128 rows a workgroup, 69 with 64, 95 with 32.
+# to 8, head_dim 128, fp16, bf16 and fp8 caches, K and V cold): the choice is 1 % above the sweep's best on average, 5 % at
+# worst (profiles/drafted_attention_launch_sweep.txt).  head_dim enters by the bytes alone, though a token of 64 is staged and
+# multiplied in less time: over 6 such shapes the choice is 3 % above the best on average, 11 % at worst.  Wide workgroups pay
+# also where they are half empty, since they have the most loads in flight: 24 rows of 10 nodes x 4 query heads a KV head x
+# 3000 tokens take 57 us with 128 rows a workgroup, 76 with 64, 93 with 32.
 _DRAFT_TILES = {16: (2, 9.6, 9.1, 2700.0, 6800.0), 32: (2, 9.8, 8.4, 5600.0, 6300.0), 64: (2, 18.4, 11.6, 2900.0, 6700.0),
                 128: (1, 16.7, 16.7, 4100.0, 9000.0)}
 _DRAFT_LAUNCH_NS = 5400.0
