@@ -84,17 +84,6 @@ __device__ __forceinline__ int draft_keys(const DraftParams& p, int b) {
   return n > 0 ? p.context_lens[b] + n : 0;
 }
 
-// Inclusive prefix sum over the lanes of a wave, all of them active: within the rows of 16, then across them.
-__device__ __forceinline__ int draft_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);     // row_shr 1, 2, 4, 8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);     // row_bcast 15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);     // row_bcast 31 into rows 2 and 3
-  return v;
-}
-
 // Work unit u of a partitioned launch -> (row, partition), the partitions that hold tokens first: the numbering of
 // unit_to_row_partition, whole partitions before the rows' last ones.  Lane l counts those of rows l * per_lane ....  Every
 // workgroup waits for this before its first load.
@@ -119,7 +108,7 @@ __device__ __forceinline__ bool draft_unit(const DraftParams& p, int u, int lane
       whole += w;
       tails += l - w;
     }
-  const int whole_to = draft_scan(whole), tails_to = draft_scan(tails);
+  const int whole_to = wave_scan(whole), tails_to = wave_scan(tails);
   const int total = __builtin_amdgcn_readlane(whole_to, 63);
   const bool tail = u >= total;
   const int want = tail ? u - total : u;

@@ -130,25 +130,6 @@ __device__ __forceinline__ double logit_weight(float l, float top, double c) {
   return l == top ? (l > -INFINITY ? 1.0 : 0.0) : finite_weight(l, top, c);
 }
 
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double dpp_or_zero(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
-  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
-// Inclusive prefix sum over the lanes of a wave, all of them active: within the rows of 16, then across them.
-__device__ __forceinline__ double wave_scan(double v) {
-  v += dpp_or_zero<0x111, 0xf>(v);          // row_shr 1, 2, 4, 8: the value that many lanes down, 0 at the row's start
-  v += dpp_or_zero<0x112, 0xf>(v);
-  v += dpp_or_zero<0x114, 0xf>(v);
-  v += dpp_or_zero<0x118, 0xf>(v);
-  v += dpp_or_zero<0x142, 0xa>(v);          // row_bcast 15 into rows 1 and 3
-  v += dpp_or_zero<0x143, 0xc>(v);          // row_bcast 31 into rows 2 and 3
-  return v;
-}
-
 // One lane's value in every lane.
 __device__ __forceinline__ double wave_at(double v, int lane) {
   const uint64_t u = __builtin_bit_cast(uint64_t, v);

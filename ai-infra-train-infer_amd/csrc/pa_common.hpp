@@ -123,4 +123,25 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_or_zero(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_zero(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = dpp_or_zero<CTRL, ROWS>((int)(uint32_t)u), hi = dpp_or_zero<CTRL, ROWS>((int)(uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// Inclusive prefix sum over the lanes of a wave, all of them active: within the rows of 16, then across them.
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp_or_zero<0x111, 0xf>(v);          // row_shr 1, 2, 4, 8: the value that many lanes down, 0 at the row's start
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);          // row_bcast 15 into rows 1 and 3
+  v += dpp_or_zero<0x143, 0xc>(v);          // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
 }  // namespace pa

@@ -18,6 +18,7 @@
 // number supplied by the caller, so a step is reproducible and needs no generator state on the
 // device: the first index j with sum_{i <= j, kept} p_i > u * (kept mass).
 // Logits tied with t* all stay (a sort keeps an implementation-defined subset of such a tie).
+#include "logit_row.hpp"
 #include "pa_common.hpp"
 #include "pa_host.hpp"
 
@@ -31,11 +32,7 @@ constexpr int kMaxChunks = 64;                 // chunks of a wave's range whose
 constexpr int kBuckets = 16;                   // key bits per pass of the threshold search: 4
 static_assert(kBuckets == kSampleWaves, "one wave adds up one bucket");
 
-// bit pattern -> unsigned key with the same order as the float value (-0 < +0 is harmless here)
-__device__ __forceinline__ uint32_t ordered_key32(float f) {
-  const uint32_t u = __float_as_uint(f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
+// bit pattern -> unsigned key with the same order as the float value, as ordered_key32 (-0 < +0 is harmless here)
 __device__ __forceinline__ uint32_t ordered_key16(uint32_t h) {
   return (h & 0x8000u) ? (~h & 0xffffu) : (h | 0x8000u);
 }
