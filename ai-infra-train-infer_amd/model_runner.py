@@ -752,7 +752,9 @@ class ModelRunner:
         reach context_len + nodes, context_lens [batch] int32 (committed tokens), num_nodes int32 [batch] or None ->
         logits [batch, nodes, vocab], the distribution after every node.  Node i's K and V are written at cache
         position context_len + i of every layer.  longest_context / mean_context: what the host knows of context_lens.
-        Ids past num_nodes can be anything (their logits mean nothing), the others belong to the vocabulary."""
+        Ids past num_nodes can be anything (their logits mean nothing), the others belong to the vocabulary.  Every row reads
+        its own context: a prefix that rows share is read once per row here, also where decode steps read it once for all of
+        them (ModelRunnerConfig.share_prefix_decode)."""
         from .speculative import draft_layout
         if self.model is None:
             raise RuntimeError("run_drafts: the runner has no model of PagedAttention layers")

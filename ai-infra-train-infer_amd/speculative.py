@@ -182,7 +182,9 @@ def paged_draft_attention(q, k_cache, v_cache, block_tables, context_lens, tree_
     """Attention of the drafted nodes q [batch, nodes, heads, head_dim] over the paged cache: node i attends to the row's
     context_lens committed tokens and to the nodes of its mask (draft_layout's tree_mask [batch or 1, nodes, words]), whose
     K and V have been written at cache positions context_len + node.  Returns [batch, nodes, heads, head_dim]; zeros for
-    nodes past num_nodes and for a node that sees nothing.
+    nodes past num_nodes and for a node that sees nothing.  Infinities and NaN in what a node sees, and in its query, come out as
+    the formula has it.  Queries of another type than a 16-bit cache's, or over an fp8 one, are multiplied as fp16 (bf16
+    exactly, fp32 to 11 bits, of any size), the K and V of a bf16 cache too then: beyond 65504 they count as infinite.
 
     A q of [batch * nodes, heads, head_dim] is taken too (and gives such an output); nodes then is the mask's.
     partition_size None: the launch policy's split of a row's tokens (the result does not depend on it beyond fp32
