@@ -259,3 +259,77 @@ def test_verification_gives_the_same_tokens_every_time(pa, gpu, dtype, top_p):
     first = call()
     for _ in range(10):
         assert all(torch.equal(x, y) for x, y in zip(call(), first))
+
+
+# ---------------------------------------------------------------------------------------------- far apart
+
+@pytest.mark.parametrize("cache,q_type", [("fp16", "fp16"), ("fp8", "bf16")])
+@pytest.mark.parametrize("rows", [16, 128])
+def test_attention_and_commit_in_a_pool_beyond_32_bit_offsets(pa, gpu, monkeypatch, cache, q_type, rows):
+    """The tokens' blocks lie at both ends of a K and a V plane of 5 GiB (fp8: 4.5 GiB)."""
+    from ai_infra_train_infer_amd import _native
+    from test_gpu_drafts import OneWidth
+    lib = OneWidth(_native.load(), rows)
+    monkeypatch.setattr(_native, "load", lambda: lib)
+    lens, nodes, hkv, dim, block = [70, 33], 6, 8, 128, 16
+    pool, sets, q = random_case(31, lens, nodes, 16, hkv, dim, block, cache, q_type)
+    each = block * hkv * dim * (1 if cache == "fp8" else 2)
+    big = (5 << 30) // each if cache == "fp16" else (9 << 29) // each
+    far = torch.tensor([b if i % 2 else big - pool.blocks + b for i, b in enumerate(range(pool.blocks))])
+    kv = torch.empty(2, 1, big, block, hkv, dim, dtype=DT[cache], device=gpu)
+    scales = [torch.ones(1, big, block, device=gpu) for _ in range(2)] if cache == "fp8" else [None, None]
+    raw = kv.view(torch.uint8).view(2, big, each)
+    for i, t in enumerate((pool.k, pool.v)):
+        raw[i, far.to(gpu)] = t.view(torch.uint8).view(pool.blocks, each).to(gpu)
+    if cache == "fp8":
+        scales[0][0, far.to(gpu)], scales[1][0, far.to(gpu)] = pool.ks.to(gpu), pool.vs.to(gpu)
+    tables = torch.where(pool.tables >= 0, far.int()[pool.tables.clamp(min=0).long()], -1).to(gpu)
+    mask = torch.stack([so.mask_words(s, nodes) for s in sets]).to(gpu)
+    k, v, near, ks, vs = pool.device(gpu)
+    layer = [None if s is None else s[0] for s in scales]
+    for part in (0, 32):
+        got = pa.paged_draft_attention(q.to(gpu), kv[0, 0], kv[1, 0], tables, i32(lens, gpu), mask, dim ** -0.5, *layer, partition_size=part)
+        want = pa.paged_draft_attention(q.to(gpu), k, v, near, i32(lens, gpu), mask, dim ** -0.5, ks, vs, partition_size=part)
+        assert torch.equal(got, want)
+    path, counts = i32([[0, 2, 5, -1, -1, -1], [0, 1, 3, 4, -1, -1]], gpu), i32([3, 4], gpu)
+    small = torch.stack([k, v])[:, None].contiguous()
+    small_scales = [s[None].clone() for s in (ks, vs)] if cache == "fp8" else [None, None]
+    a = pa.commit_drafts(kv, tables, i32(lens, gpu), path, counts, *scales)
+    b = pa.commit_drafts(small, near, i32(lens, gpu), path, counts, *small_scales)
+    assert torch.equal(a, b)
+    assert torch.equal(raw[:, far.to(gpu)], small.view(torch.uint8).view(2, pool.blocks, each))
+    if cache == "fp8":
+        for x, y in zip(scales, small_scales):
+            assert torch.equal(x[0, far.to(gpu)].nan_to_num(7.0), y[0].nan_to_num(7.0))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_verification_of_rows_beyond_32_bit_offsets(pa, gpu, dtype):
+    """Logits and draft probabilities whose rows are 2^30 entries and whose sequences 2^32 bytes and more apart."""
+    g = torch.Generator().manual_seed(37)
+    vocab, nodes, batch = 1003, 3, 2
+    near = (torch.randn(batch, nodes, vocab, generator=g) * 2).to(DT[dtype]).to(gpu)
+    q_near = torch.softmax(near[:, :-1].float() + 0.5 * torch.randn(batch, nodes - 1, vocab, generator=g).to(gpu), -1)
+    tokens = torch.cat([torch.zeros(batch, 1, dtype=torch.long), torch.multinomial(q_near.cpu().view(-1, vocab), 1, generator=g).view(batch, -1)], 1).to(gpu)
+    u = torch.rand(batch, nodes, generator=g).to(gpu)
+    row, seq = (1 << 30) + 1, 3 * (1 << 30) + 7
+    flat = torch.empty(seq + 2 * row + vocab, dtype=DT[dtype], device=gpu)
+    far = flat.as_strided(near.shape, (seq, row, 1))
+    far.copy_(near)
+    q_flat = torch.empty(seq + row + vocab, device=gpu)
+    q_far = q_flat.as_strided(q_near.shape, (seq, row, 1))
+    q_far.copy_(q_near)
+    for kw_far, kw_near in ((dict(), dict()), (dict(draft_probs=q_far), dict(draft_probs=q_near))):
+        for temperature, top_p in ((0.0, 1.0), (0.9, 0.9), (1.0, 1.0)):
+            a = pa.verify_drafts(far, tokens, u, temperature=temperature, top_p=top_p, **kw_far)
+            b = pa.verify_drafts(near, tokens, u, temperature=temperature, top_p=top_p, **kw_near)
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("temperature", [1e-6, 1e-3, 50.0, 1e6])
+@pytest.mark.parametrize("top_p", [1.0, 0.9, 0.5])
+def test_verify_at_extreme_temperatures(pa, gpu, dtype, temperature, top_p):
+    """From one token that takes everything to weights that differ in the seventh digit."""
+    check_verify(pa, gpu, 41, 6, 7, 331, dtype, temperature, top_p)
+    check_verify(pa, gpu, 42, 4, 4, 17003, dtype, temperature, top_p, kind="chain", probs="fp32")
